@@ -116,6 +116,74 @@ SIGNATURES = {
     ),
 }
 
+# Constants and functions of include/mlxc_train.h.
+MLXC_FLOAT32 = 0
+MLXC_BFLOAT16 = 1
+MLXC_FLOAT16 = 2
+MLXC_GRAD_SPARSE = 1
+MLXC_PREFERENCE_NORMALIZE = 1
+MLXC_PREFERENCE_SUM = 2
+
+
+class PreferenceSide(ctypes.Structure):
+    """mlxc_preference_side."""
+    _fields_ = [("values", _ptr), ("reference", _ptr), ("mask", _ptr), ("length", _i64),
+                ("grad", _ptr)]
+
+
+_side = ctypes.POINTER(PreferenceSide)
+_flt = ctypes.c_float
+
+# name -> (restype, argtypes); every function include/mlxc_train.h declares.
+TRAIN_SIGNATURES = {
+    "mlxc_embedding": (
+        ctypes.c_int,
+        [_ptr, _i64, _i32, _i64, _i32, _ptr, _i64, _i32, _flt, _ptr, _ptr, _ptr],
+    ),
+    "mlxc_embedding_grad_workspace_bytes": (_size, [_i64, _i32, _i64, _i32]),
+    "mlxc_embedding_grad": (
+        ctypes.c_int,
+        [_ptr, _i32, _i32, _ptr, _i64, _i32, _i64, _flt, _i32, _ptr, _ptr, _i32, _ptr, _size,
+         _ptr],
+    ),
+    "mlxc_window_scores": (
+        ctypes.c_int,
+        [_ptr, _i64, _i32, _i64, _i32, _ptr, _i64, _i32, _i32, _i32, _flt, _ptr, _ptr, _ptr],
+    ),
+    "mlxc_window_scores_grad_workspace_bytes": (_size, [_i64, _i32, _i64, _i32, _i32, _i32]),
+    "mlxc_window_scores_grad": (
+        ctypes.c_int,
+        [_ptr, _ptr, _i64, _i32, _i64, _i32, _ptr, _i64, _i32, _i32, _i32, _flt, _i32, _ptr, _ptr,
+         _i32, _ptr, _size, _ptr],
+    ),
+    "mlxc_preference_loss_workspace_bytes": (_size, [_i64]),
+    "mlxc_preference_loss": (
+        ctypes.c_int,
+        [_side, _side, _i64, _i32, _flt, _flt, _i32, _ptr, _ptr, _ptr, _ptr, _size, _ptr],
+    ),
+    "mlxc_preference_grad": (ctypes.c_int, [_side, _side, _i64, _i32, _ptr, _ptr, _ptr]),
+    "mlxc_embedding_cpu": (
+        ctypes.c_int, [_ptr, _i64, _i32, _i64, _i32, _ptr, _i64, _i32, _flt, _ptr, _ptr],
+    ),
+    "mlxc_embedding_grad_cpu": (
+        ctypes.c_int,
+        [_ptr, _i32, _i32, _ptr, _i64, _i32, _i64, _flt, _i32, _ptr, _ptr, _i32, _ptr],
+    ),
+    "mlxc_window_scores_cpu": (
+        ctypes.c_int,
+        [_ptr, _i64, _i32, _i64, _i32, _ptr, _i64, _i32, _i32, _i32, _flt, _ptr, _ptr],
+    ),
+    "mlxc_window_scores_grad_cpu": (
+        ctypes.c_int,
+        [_ptr, _ptr, _i64, _i32, _i64, _i32, _ptr, _i64, _i32, _i32, _i32, _flt, _i32, _ptr, _ptr,
+         _i32, _ptr],
+    ),
+    "mlxc_preference_loss_cpu": (
+        ctypes.c_int, [_side, _side, _i64, _i32, _flt, _flt, _i32, _ptr, _ptr, _ptr],
+    ),
+    "mlxc_preference_grad_cpu": (ctypes.c_int, [_side, _side, _i64, _i32, _ptr, _ptr]),
+}
+
 _lib = None
 
 
@@ -129,7 +197,7 @@ def load() -> ctypes.CDLL:
             f"{LIB_PATH} is not built; run `python -m mlx_cluster_amd.build_lib` "
             "(this package has no CPU fallback)")
     lib = ctypes.CDLL(LIB_PATH)
-    for name, (res, args) in SIGNATURES.items():
+    for name, (res, args) in {**SIGNATURES, **TRAIN_SIGNATURES}.items():
         fn = getattr(lib, name)
         fn.restype = res
         fn.argtypes = args

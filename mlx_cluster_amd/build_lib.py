@@ -15,7 +15,9 @@ REPO_DIR = os.path.dirname(PKG_DIR)
 CSRC = os.path.join(PKG_DIR, "csrc")
 SOURCES = [os.path.join(CSRC, f) for f in
            ("mlxc_api.hip", "prep_kernels.hip", "uniform_walk.hip", "node2vec_walk.hip",
-            "csr_build.hip", "windows.hip", "gather_probe.hip", "host_walk.cpp", "host_csr.cpp")]
+            "csr_build.hip", "windows.hip", "gather_probe.hip", "train_api.hip", "embedding.hip",
+            "window_scores.hip", "preference.hip", "host_walk.cpp", "host_csr.cpp",
+            "host_train.cpp")]
 OUT = os.path.join(PKG_DIR, "libmlxc.so")
 INCLUDE = os.path.join(REPO_DIR, "include")
 
@@ -110,7 +112,7 @@ def build_binding(verbose: bool = False, lib: str = OUT) -> str:
 def source_files() -> list[str]:
     """Every file the library is built from (kernels, headers, C ABI)."""
     return sorted([os.path.join(CSRC, f) for f in os.listdir(CSRC)] +
-                  [os.path.join(INCLUDE, "mlxc.h")])
+                  [os.path.join(INCLUDE, f) for f in ("mlxc.h", "mlxc_train.h")])
 
 
 def _code_only(text: str) -> str:
