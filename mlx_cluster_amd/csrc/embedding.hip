@@ -7,12 +7,12 @@
 // The gradient sorts (node, place) by node, stable, with an LSD radix sort of
 // the bits that a node can have, so that a node's places stand together in
 // ascending order; then every row adds its places up.  Places without a node
-// are dropped by the first pass.  Walks visit hubs tens of thousands of times:
-// the sorted places are cut into tiles of 64, tiles of 64 tiles and so on, a
-// tile that lies in one node's run is added up once by the tile kernels, and
-// the row takes its sum instead of its places.  So no lane adds more than a few
-// hundred rows, nothing is added with atomics, and the order of a sum depends
-// on the places alone.
+// are dropped by the first pass.  Walks visit hubs tens of thousands of times,
+// so the sorted places are added up in tiles of 32, each by one group of lanes
+// whatever runs it holds; a run that crosses tiles is put together from its
+// tiles' parts, a hub's from sums of 16 tiles, of 16 of these, and so on.  So no
+// lane adds more than a few dozen rows, nothing is added with atomics, and the
+// order of a sum depends on the places alone.
 #include "train_host.h"
 
 namespace mlxc {
@@ -58,9 +58,7 @@ constexpr int kWaves = kBlock / kWave;
 constexpr int kWaveTile = kWave * kItems;
 static_assert(kDigits == kBlock, "one digit a thread");
 
-// Words of the workspace header.
-constexpr int kWordStatus = 0;
-constexpr int kWordDistinct = 1;  // distinct nodes (coalesced)
+constexpr int kWordStatus = 0;  // of the workspace header
 
 // Exclusive prefix of one value a thread over the block; *total the sum.  `tot`
 // is kWaves words of LDS.  Contains two barriers.
@@ -228,19 +226,11 @@ __global__ __launch_bounds__(kBlock) void digit_scatter_kernel(
 
 // ------------------------------------------------------------- runs
 
-// Dense: the run of every node that occurs, [runs[v].x, runs[v].y) of the
-// sorted places; runs is zeroed before.
-__global__ __launch_bounds__(kBlock) void mark_runs_kernel(const uint32_t* __restrict__ keys,
-                                                           const uint32_t* __restrict__ valid,
-                                                           uint2* __restrict__ runs) {
-    const int64_t n = *valid;
-    for (int64_t i = blockIdx.x * static_cast<int64_t>(kBlock) + threadIdx.x; i < n;
-         i += static_cast<int64_t>(gridDim.x) * kBlock) {
-        const uint32_t k = keys[i];
-        if (i == 0 || keys[i - 1] != k) runs[k].x = static_cast<uint32_t>(i);
-        if (i == n - 1 || keys[i + 1] != k) runs[k].y = static_cast<uint32_t>(i + 1);
-    }
-}
+// The sorted places are added up in tiles of kSpan.  Level 1's tiles hold kFan
+// of these, level l's kFan^l.
+constexpr int kSpan = 32;
+constexpr int kFan = 16;
+constexpr int kMaxLevels = 6;
 
 // Coalesced: heads[chunk] <- the runs that start in a chunk of kTile places.
 __global__ __launch_bounds__(kBlock) void count_heads_kernel(const uint32_t* __restrict__ keys,
@@ -258,13 +248,13 @@ __global__ __launch_bounds__(kBlock) void count_heads_kernel(const uint32_t* __r
     if (threadIdx.x == 0) heads[blockIdx.x] = all;
 }
 
-// ... and run u's start, its node, and the number of runs.
+// ... then the runs' nodes, and ranks[p] <- the runs that start before tile p
+// of kSpan places.
 __global__ __launch_bounds__(kBlock) void list_runs_kernel(const uint32_t* __restrict__ keys,
                                                            const uint32_t* __restrict__ valid,
                                                            const uint32_t* __restrict__ heads,
-                                                           uint32_t* __restrict__ starts,
-                                                           int64_t* __restrict__ ids,
-                                                           int64_t* __restrict__ work) {
+                                                           uint32_t* __restrict__ ranks,
+                                                           int64_t* __restrict__ ids) {
     __shared__ uint32_t tot[kWaves];
     const int64_t n = *valid, base = static_cast<int64_t>(blockIdx.x) * kTile;
     uint32_t part = 0, before;
@@ -278,20 +268,13 @@ __global__ __launch_bounds__(kBlock) void list_runs_kernel(const uint32_t* __res
     }
     uint32_t all;
     uint32_t u = before + block_prefix(__popc(is_head), tot, &all);
-    for (int s = 0; s < kItems; ++s) {
-        if (!((is_head >> s) & 1)) continue;
-        starts[u] = static_cast<uint32_t>(first + s);
-        ids[u++] = keys[first + s];
-    }
-    if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) work[kWordDistinct] = before + all;
+    static_assert(kSpan % kItems == 0, "a tile starts with a thread's places");
+    if (first % kSpan == 0 && first < n) ranks[first / kSpan] = u;
+    for (int s = 0; s < kItems; ++s)
+        if ((is_head >> s) & 1) ids[u++] = keys[first + s];
 }
 
 // ------------------------------------------------------------- sums
-
-// Tile sums: level l's tile p covers the sorted places [p * 64^l, (p + 1) *
-// 64^l), for l = 1 .. levels.
-constexpr int kFan = 64;
-constexpr int kMaxLevels = 3;
 
 // The lanes that serve one row: 2^lanes_log of them, a pack of N columns each,
 // from column first_column on.
@@ -300,36 +283,160 @@ struct RowShape {
     int32_t lanes_log;
 };
 
-template <typename E, int N>
-__device__ __forceinline__ void add_row(float (&acc)[N], const typename E::S* row) {
-    float x[N];
-    load_pack<E, N>(x, row);
+// acc += rows index(from) .. index(to - 1), in order; kBatch loads in flight, those
+// past the end of the last row again, and added as zeros: added behind a branch,
+// they are moved there by the compiler, one load after the other (a batch then
+// takes 12.7 us instead of 2).
+#ifndef MLXC_SUM_BATCH
+#define MLXC_SUM_BATCH 8
+#endif
+constexpr int kBatch = MLXC_SUM_BATCH;
+template <typename E, int N, typename Index>
+__device__ __forceinline__ void add_rows(float (&acc)[N], const typename E::S* __restrict__ rows,
+                                         int32_t dim, int32_t col, int64_t from, int64_t to,
+                                         Index index) {
+    for (int64_t q = from; q < to; q += kBatch) {
+        int64_t r[kBatch];
 #pragma unroll
-    for (int q = 0; q < N; ++q) acc[q] += x[q];
+        for (int u = 0; u < kBatch; ++u) r[u] = index(q + u < to ? q + u : to - 1);
+        Pack<typename E::S, N> x[kBatch];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u)
+            x[u] = *reinterpret_cast<const Pack<typename E::S, N>*>(rows + r[u] * dim + col);
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u)
+            for (int k = 0; k < N; ++k) {
+                const float y = E::load(x[u].v[k]);
+                acc[k] += q + u < to ? y : 0.f;
+            }
+    }
 }
 
-// sums[p, :] <- the sum of tile p's kFan rows (level 1: the rows of its places,
-// E; above: the level below's sums) where the tile lies in one run.
-template <typename E, int N, bool kRows>
-__global__ __launch_bounds__(kBlock) void tile_sum_kernel(
-    const uint32_t* __restrict__ keys, const uint32_t* __restrict__ valid, int64_t span,
-    const typename E::S* __restrict__ rows, const uint32_t* __restrict__ places, RowShape shape,
-    float* __restrict__ sums) {
+// Keeps a loaded pack's load where it stands.
+template <typename S, int N>
+__device__ __forceinline__ void pin(Pack<S, N>& p) {
+    if constexpr (sizeof(S) * N == 4) {
+        uint32_t w = __builtin_bit_cast(uint32_t, p);
+        asm volatile("" : "+v"(w));
+        p = __builtin_bit_cast(Pack<S, N>, w);
+    } else if constexpr (sizeof(S) * N > 4) {
+        typedef uint32_t Words __attribute__((ext_vector_type(sizeof(S) * N / 4)));
+        Words w = __builtin_bit_cast(Words, p);
+        asm volatile("" : "+v"(w));
+        p = __builtin_bit_cast(Pack<S, N>, w);
+    } else {
+        asm volatile("" : "+v"(p.v[0]));
+    }
+}
+
+// The sums of one call: where the parts of runs that cross tiles go.
+struct Parts {
+    float* first;  // [tiles, dim] the part of a run that enters the tile, or fills it
+    float* last;   // [tiles, dim] the part of a run that leaves it, where it did not enter it
+};
+
+// A group of lanes adds up the kSpan places of a tile, kBatch rows in flight
+// whatever runs they belong to, and stores a run that lies in the tile as the
+// row it is; parts of others go to `parts`.  So the gather is spread evenly
+// however often a node occurs.  Marks the runs by output row: the node, or
+// (ranks given) its rank among the nodes.
+template <typename E, typename O, int N>
+__global__ __launch_bounds__(kBlock) void span_sum_kernel(
+    const typename E::S* __restrict__ rows, const uint32_t* __restrict__ keys,
+    const uint32_t* __restrict__ places, const uint32_t* __restrict__ valid,
+    const uint32_t* __restrict__ ranks, RowShape shape, float scale, Parts parts,
+    uint2* __restrict__ runs, typename O::S* __restrict__ out) {
     const int lane = threadIdx.x & ((1 << shape.lanes_log) - 1);
-    const int64_t groups = static_cast<int64_t>(gridDim.x) * (kBlock >> shape.lanes_log);
     const int32_t col = ((blockIdx.y << shape.lanes_log) + lane) * N;
+    if (col >= shape.dim) return;
+    const int64_t groups = static_cast<int64_t>(gridDim.x) * (kBlock >> shape.lanes_log);
+    const bool marks = lane == 0 && blockIdx.y == 0;
     const int64_t n = *valid;
     for (int64_t p = (blockIdx.x * static_cast<int64_t>(kBlock) + threadIdx.x) >> shape.lanes_log;
-         (p + 1) * span <= n; p += groups) {
-        if (keys[p * span] != keys[(p + 1) * span - 1] || col >= shape.dim) continue;
+         p * kSpan < n; p += groups) {
+        const int64_t begin = p * kSpan;
+        const int64_t end = begin + kSpan < n ? begin + kSpan : n;
+        uint32_t node = keys[begin];
+        const bool enters = begin > 0 && keys[begin - 1] == node;
+        int64_t rank = ranks ? static_cast<int64_t>(ranks[p]) - enters : 0;
+        if (marks && !enters) runs[ranks ? rank : node].x = static_cast<uint32_t>(begin);
+        bool first = true;  // no run has ended in the tile yet
         float acc[N] = {};
-#pragma unroll 4
-        for (int q = 0; q < kFan; ++q) {
-            const int64_t r = kRows ? static_cast<int64_t>(places[p * kFan + q]) : p * kFan + q;
-            add_row<E, N>(acc, rows + r * shape.dim + col);
+        for (int64_t i = begin; i < end; i += kBatch) {
+            uint32_t key[kBatch];
+            Pack<typename E::S, N> x[kBatch];
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) {
+                const int64_t at = i + u < end ? i + u : end - 1;
+                key[u] = keys[at];
+                x[u] = *reinterpret_cast<const Pack<typename E::S, N>*>(
+                    rows + static_cast<int64_t>(places[at]) * shape.dim + col);
+            }
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) pin(x[u]);
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) {
+                if (key[u] != node) {
+                    const int64_t row = ranks ? rank : static_cast<int64_t>(node);
+                    if (first && enters) {
+                        store_pack<F32, N>(parts.first + p * shape.dim + col, acc);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < N; ++k) acc[k] *= scale;
+                        store_pack<O, N>(out + row * shape.dim + col, acc);
+                    }
+                    if (marks) {
+                        runs[row].y = static_cast<uint32_t>(i + u);
+                        runs[ranks ? rank + 1 : static_cast<int64_t>(key[u])].x =
+                            static_cast<uint32_t>(i + u);
+                    }
+                    first = false;
+                    node = key[u];
+                    ++rank;
+#pragma unroll
+                    for (int k = 0; k < N; ++k) acc[k] = 0.f;
+                }
+#pragma unroll
+                for (int k = 0; k < N; ++k) {
+                    const float y = E::load(x[u].v[k]);
+                    acc[k] += i + u < end ? y : 0.f;
+                }
+            }
         }
-        store_pack<F32, N>(sums + p * shape.dim + col, acc);
+        const bool leaves = end < n && keys[end] == node;
+        const int64_t row = ranks ? rank : static_cast<int64_t>(node);
+        if (first && enters) {
+            store_pack<F32, N>(parts.first + p * shape.dim + col, acc);
+        } else if (leaves) {
+            store_pack<F32, N>((first ? parts.first : parts.last) + p * shape.dim + col, acc);
+        } else {
+#pragma unroll
+            for (int k = 0; k < N; ++k) acc[k] *= scale;
+            store_pack<O, N>(out + row * shape.dim + col, acc);
+        }
+        if (marks && !leaves) runs[row].y = static_cast<uint32_t>(end);
     }
+}
+
+// sums[p, :] <- the sum of kFan entries of the level below, for the tiles of
+// `span` places that lie in one run.
+template <int N>
+__global__ __launch_bounds__(kBlock) void tile_sum_kernel(const uint32_t* __restrict__ keys,
+                                                          const uint32_t* __restrict__ valid,
+                                                          int64_t span,
+                                                          const float* __restrict__ below,
+                                                          RowShape shape,
+                                                          float* __restrict__ sums) {
+    const int lane = threadIdx.x & ((1 << shape.lanes_log) - 1);
+    const int32_t col = ((blockIdx.y << shape.lanes_log) + lane) * N;
+    const int64_t p =
+        (blockIdx.x * static_cast<int64_t>(kBlock) + threadIdx.x) >> shape.lanes_log;
+    if ((p + 1) * span > *valid || keys[p * span] != keys[(p + 1) * span - 1] || col >= shape.dim)
+        return;
+    float acc[N] = {};
+    add_rows<F32, N>(acc, below, shape.dim, col, p * kFan, (p + 1) * kFan,
+                     [](int64_t q) { return q; });
+    store_pack<F32, N>(sums + p * shape.dim + col, acc);
 }
 
 struct TileSums {
@@ -337,51 +444,68 @@ struct TileSums {
     int32_t levels;
 };
 
-// Every row of the output: scale * the sum of its run, tiles where they lie in
-// it whole.  Dense: row v's run is runs[v]; coalesced: run u is [starts[u],
-// starts[u + 1]), and past the last run rows are zeros and ids -1.
-template <typename E, typename O, int N>
+constexpr int kZeroBlocks = 16;  // a compute unit, of the blocks that write zeros
+
+// What span_sum_kernel left.  The first `finish` blocks put the runs that cross
+// tiles together, each by the group of the tile in which it starts: neighbouring
+// nodes, and those a power of two apart, are often hubs together, and a group a
+// row adds up one hub after the other (2^20 rows of 128 bfloat16: 153 us; so
+// @ROWUS@).  The others write zeros where a row has no run (and its id, -1, if
+// the call lists ids).
+template <typename O, int N>
 __global__ __launch_bounds__(kBlock) void row_sum_kernel(
-    const typename E::S* __restrict__ rows, const uint32_t* __restrict__ places,
-    const uint32_t* __restrict__ valid, const uint2* __restrict__ runs,
-    const uint32_t* __restrict__ starts, const int64_t* __restrict__ work, int64_t* __restrict__ ids,
-    TileSums tiles, RowShape shape, int64_t num_out, float scale, typename O::S* __restrict__ out) {
+    const uint32_t* __restrict__ keys, const uint32_t* __restrict__ valid,
+    const uint32_t* __restrict__ ranks, const uint2* __restrict__ runs, Parts parts, TileSums tiles,
+    RowShape shape, unsigned finish, int64_t num_out, float scale, int64_t* __restrict__ ids,
+    typename O::S* __restrict__ out) {
     const int lane = threadIdx.x & ((1 << shape.lanes_log) - 1);
-    const int64_t groups = static_cast<int64_t>(gridDim.x) * (kBlock >> shape.lanes_log);
+    const int64_t per = kBlock >> shape.lanes_log;  // groups a block
+    const int64_t own = threadIdx.x >> shape.lanes_log;
     const int32_t col = ((blockIdx.y << shape.lanes_log) + lane) * N;
-    const int64_t distinct = ids ? work[kWordDistinct] : 0;
-    for (int64_t v = (blockIdx.x * static_cast<int64_t>(kBlock) + threadIdx.x) >> shape.lanes_log;
-         v < num_out; v += groups) {
-        int64_t i = 0, end = 0;
-        if (!ids) {
-            const uint2 r = runs[v];
-            i = r.x;
-            end = r.y;
-        } else if (v < distinct) {
-            i = starts[v];
-            end = v + 1 < distinct ? starts[v + 1] : *valid;
-        } else if (lane == 0 && blockIdx.y == 0) {
-            ids[v] = -1;
+    if (blockIdx.x >= finish) {
+        const int64_t groups = (gridDim.x - finish) * per;
+        for (int64_t v = (blockIdx.x - finish) * per + own; v < num_out; v += groups) {
+            const uint2 run = runs[v];
+            if (run.x != run.y) continue;
+            if (ids && lane == 0 && blockIdx.y == 0) ids[v] = -1;
+            const float zeros[N] = {};
+            if (col < shape.dim) store_pack<O, N>(out + v * shape.dim + col, zeros);
         }
-        if (col >= shape.dim) continue;
+        return;
+    }
+    if (col >= shape.dim) return;
+    const int64_t n = *valid;
+    for (int64_t p = blockIdx.x * per + own; (p + 1) * kSpan < n; p += finish * per) {
+        const uint32_t node = keys[(p + 1) * kSpan - 1];
+        const bool leaves = keys[(p + 1) * kSpan] == node;
+        const bool entered = p > 0 && keys[p * kSpan - 1] == node;
+        if (!leaves || entered) continue;
+        const int64_t row = ranks ? static_cast<int64_t>(ranks[p + 1]) - 1 : node;
+        const uint2 run = runs[row];
         float acc[N] = {};
-        while (i < end) {
-            // the largest tile that starts here and lies in the run
-            int64_t span = 1;
-            int level = 0;
-            while (level < tiles.levels && i % (span * kFan) == 0 && i + span * kFan <= end) {
-                span *= kFan;
-                ++level;
-            }
-            if (level == 0)
-                add_row<E, N>(acc, rows + static_cast<int64_t>(places[i]) * shape.dim + col);
-            else
-                add_row<F32, N>(acc, tiles.p[level - 1] + i / span * shape.dim + col);
-            i += span;
+        int64_t lo = p, hi = (run.y - 1) / kSpan + 1;  // the run's tiles
+        if (run.x % kSpan) {  // it starts inside its first tile
+            load_pack<F32, N>(acc, parts.last + lo * shape.dim + col);
+            ++lo;
+        }
+        // the parts before the first whole tile of tiles and after the last
+        // one, then the same a level up; parts from `full` on are not whole
+        int64_t full = run.y / kSpan;
+        for (int level = 0;; ++level) {
+            const int64_t first = (lo + kFan - 1) / kFan, last = full / kFan;
+            const bool more = level < tiles.levels && first < last;
+            const int64_t head = more ? first * kFan - lo : hi - lo;
+            const int64_t tail = more ? last * kFan - head : 0;  // of entry head on
+            const int64_t count = more ? head + hi - last * kFan : head;
+            add_rows<F32, N>(acc, level == 0 ? parts.first : tiles.p[level - 1], shape.dim, col, 0,
+                             count, [&](int64_t q) { return q < head ? lo + q : tail + q; });
+            if (!more) break;
+            lo = first;
+            hi = full = last;
         }
 #pragma unroll
-        for (int q = 0; q < N; ++q) acc[q] *= scale;
-        store_pack<O, N>(out + v * shape.dim + col, acc);
+        for (int k = 0; k < N; ++k) acc[k] *= scale;
+        store_pack<O, N>(out + row * shape.dim + col, acc);
     }
 }
 
@@ -402,7 +526,8 @@ int bits_below(int64_t n) {  // bits of n - 1
 struct GradLayout {
     int passes = 1;
     uint32_t tiles = 0;
-    size_t keys[2], places[2], counts, totals, valid, runs, heads, sums[kMaxLevels], bytes;
+    size_t keys[2], places[2], counts, totals, valid, runs, heads, ranks, first, last;
+    size_t sums[kMaxLevels], bytes;
     int levels = 0;
 };
 
@@ -424,10 +549,14 @@ GradLayout grad_layout(int64_t num_rows, int32_t dim, int64_t count, bool sparse
     l.counts = take(static_cast<size_t>(l.tiles) * kDigits * 4);
     l.totals = take(kDigits * 4);
     l.valid = take(8);
-    const int64_t cap = count < num_rows ? count : num_rows;
-    l.runs = take(static_cast<size_t>(sparse ? cap * 4 : num_rows * 8));
+    const int64_t num_out = sparse && count < num_rows ? count : num_rows;
+    const int64_t spans = (count + kSpan - 1) / kSpan;
+    l.runs = take(static_cast<size_t>(num_out) * sizeof(uint2));
     l.heads = take(static_cast<size_t>(sparse ? l.tiles : 0) * 4);
-    for (int64_t span = kFan; l.levels < kMaxLevels && span <= count; span *= kFan)
+    l.ranks = take(static_cast<size_t>(sparse ? spans : 0) * 4);
+    l.first = take(static_cast<size_t>(spans) * dim * 4);
+    l.last = take(static_cast<size_t>(spans) * dim * 4);
+    for (int64_t span = kSpan * kFan; l.levels < kMaxLevels && span <= count; span *= kFan)
         l.sums[l.levels++] = take(static_cast<size_t>(count / span) * dim * 4);
     l.bytes = at;
     return l;
@@ -444,12 +573,13 @@ RowShape row_shape(int32_t dim, int n) {
     return s;
 }
 
-// Blocks for `rows` rows of this shape, and the columns' share of the grid.
-dim3 row_grid(int64_t rows, const RowShape& s, int n, int cus) {
+// Blocks for `rows` rows of this shape (fewer where a launch would hold 2^32
+// threads: the kernels go on by the grid's groups), and the columns' share of
+// the grid.
+dim3 row_grid(int64_t rows, const RowShape& s, int n) {
     const int64_t per = kBlock >> s.lanes_log;
     int64_t blocks = (rows + per - 1) / per;
-    const int64_t most = static_cast<int64_t>(cus) * 64;
-    if (blocks > most) blocks = most;
+    if (blocks > (1 << 23)) blocks = 1 << 23;
     const int32_t cols = n << s.lanes_log;
     return dim3(static_cast<unsigned>(blocks < 1 ? 1 : blocks), (s.dim + cols - 1) / cols);
 }
@@ -483,43 +613,51 @@ struct SumCall {
 
 template <typename E, typename O, int N>
 int sums_typed(const SumCall& c, hipStream_t stream) {
-    DeviceInfo info;
-    if (int rc = device_info(info)) return rc;
     const RowShape shape = row_shape(c.dim, N);
+    const Parts parts{at<float>(c.ws, c.l.first), at<float>(c.ws, c.l.last)};
+    uint2* runs = at<uint2>(c.ws, c.l.runs);
+    const uint32_t* ranks = c.out.ids ? at<const uint32_t>(c.ws, c.l.ranks) : nullptr;
+    typename O::S* out = static_cast<typename O::S*>(c.out.p);
+    if (c.count > 0) {
+        hipLaunchKernelGGL((span_sum_kernel<E, O, N>),
+                           row_grid((c.count + kSpan - 1) / kSpan, shape, N), dim3(kBlock), 0,
+                           stream, static_cast<const typename E::S*>(c.rows), c.keys, c.places,
+                           c.valid, ranks, shape, c.scale, parts, runs, out);
+        MLXC_HIP_TRY(hipGetLastError());
+    }
     TileSums tiles{};
-    int64_t span = 1;
+    int64_t span = kSpan;
     for (int k = 0; k < c.l.levels; ++k) {
         span *= kFan;
         float* sums = at<float>(c.ws, c.l.sums[k]);
-        const dim3 grid = row_grid(c.count / span, shape, N, info.cus);
-        if (k == 0)
-            hipLaunchKernelGGL((tile_sum_kernel<E, N, true>), grid, dim3(kBlock), 0, stream, c.keys,
-                               c.valid, span, static_cast<const typename E::S*>(c.rows), c.places,
-                               shape, sums);
-        else
-            hipLaunchKernelGGL((tile_sum_kernel<F32, N, false>), grid, dim3(kBlock), 0, stream,
-                               c.keys, c.valid, span, tiles.p[k - 1], nullptr, shape, sums);
+        hipLaunchKernelGGL((tile_sum_kernel<N>), row_grid(c.count / span, shape, N), dim3(kBlock), 0,
+                           stream, c.keys, c.valid, span, k == 0 ? parts.first : tiles.p[k - 1],
+                           shape, sums);
         MLXC_HIP_TRY(hipGetLastError());
         tiles.p[k] = sums;
         tiles.levels = k + 1;
     }
-    hipLaunchKernelGGL((row_sum_kernel<E, O, N>), row_grid(c.num_out, shape, N, info.cus),
-                       dim3(kBlock), 0, stream, static_cast<const typename E::S*>(c.rows), c.places,
-                       c.valid, at<const uint2>(c.ws, c.l.runs), at<const uint32_t>(c.ws, c.l.runs),
-                       static_cast<const int64_t*>(c.ws), c.out.ids, tiles, shape, c.num_out,
-                       c.scale, static_cast<typename O::S*>(c.out.p));
+    DeviceInfo info;
+    if (int rc = device_info(info)) return rc;
+    const dim3 finish = row_grid(c.count / kSpan, shape, N);
+    dim3 grid = row_grid(c.num_out, shape, N);
+    const unsigned most = info.cus * kZeroBlocks;
+    grid.x = finish.x + (grid.x < most ? grid.x : most);
+    hipLaunchKernelGGL((row_sum_kernel<O, N>), grid, dim3(kBlock), 0, stream, c.keys, c.valid,
+                       ranks, runs, parts, tiles, shape, finish.x, c.num_out, c.scale, c.out.ids,
+                       out);
     MLXC_HIP_TRY(hipGetLastError());
     return MLXC_OK;
 }
 
 template <typename E, typename O>
 int sums_packed(const SumCall& c, hipStream_t stream) {
-    constexpr size_t esz = sizeof(typename E::S), osz = sizeof(typename O::S);
-    // a pack is at most 16 bytes of either; the tiles' sums follow the packs,
-    // their rows aligned as dim says
-    constexpr int most = 16 / (esz > osz ? esz : osz);
-    const int n = pack_width(c.rows, c.dim, c.dim, esz, most);
-    const int m = pack_width(c.out.p, c.dim, c.dim, osz, n < 4 ? n : 4);
+    // a pack of up to 16 bytes of the rows; its sums and results are stored in
+    // one or two instructions, which the same alignment serves
+    constexpr int most = 16 / sizeof(typename E::S);
+    const int n = pack_width(c.rows, c.dim, c.dim, sizeof(typename E::S), most);
+    const int m = pack_width(c.out.p, c.dim, c.dim, sizeof(typename O::S), n);
+    if (m >= 8) return sums_typed<E, O, most>(c, stream);
     if (m >= 4) return sums_typed<E, O, 4>(c, stream);
     if (m >= 2) return sums_typed<E, O, 2>(c, stream);
     return sums_typed<E, O, 1>(c, stream);
@@ -595,7 +733,7 @@ int launch_embedding_grad(const void* rows, int32_t dtype, int32_t dim, const No
                  *places_out = at<uint32_t>(workspace, l.places[to]);
         if (pass == 0) {
             hipLaunchKernelGGL(digit_count_kernel<true>, dim3(blocks), dim3(kBlock), 0, stream, in,
-                               shift, l.tiles, counts, runs, sparse ? 0 : 2 * nodes.num_rows, work);
+                               shift, l.tiles, counts, runs, 2 * num_out, work);
         } else {
             hipLaunchKernelGGL(digit_count_kernel<false>, dim3(blocks), dim3(kBlock), 0, stream, in,
                                shift, l.tiles, counts, nullptr, 0, work);
@@ -618,12 +756,9 @@ int launch_embedding_grad(const void* rows, int32_t dtype, int32_t dim, const No
                            heads);
         MLXC_HIP_TRY(hipGetLastError());
         hipLaunchKernelGGL(list_runs_kernel, dim3(blocks), dim3(kBlock), 0, stream, keys, valid,
-                           heads, runs, out.ids, work);
-    } else {
-        hipLaunchKernelGGL(mark_runs_kernel, dim3(blocks * 4), dim3(kBlock), 0, stream, keys, valid,
-                           reinterpret_cast<uint2*>(runs));
+                           heads, at<uint32_t>(workspace, l.ranks), out.ids);
+        MLXC_HIP_TRY(hipGetLastError());
     }
-    MLXC_HIP_TRY(hipGetLastError());
     const SumCall c{keys, places, valid, rows, dim, count, num_out, scale, l, workspace, out};
     if (dtype == MLXC_FLOAT32) return sums_from<F32>(c, stream);
     if (dtype == MLXC_BFLOAT16) return sums_from<BF16>(c, stream);
