@@ -124,7 +124,7 @@ typedef struct mlxc_preference_side {
     const void* values;    /* [pairs, length] log-probabilities or scores */
     const void* reference; /* [pairs, length] of the reference model, or NULL (zeros) */
     const uint8_t* mask;   /* [pairs, length], 0 leaves a value out, or NULL (none left out) */
-    int64_t length;        /* [0, 2^31) */
+    int64_t length;        /* [0, 2^30) */
     void* grad;            /* [pairs, length] of dtype, or NULL (not wanted) */
 } mlxc_preference_side;
 

@@ -112,7 +112,8 @@ int check_preference(const mlxc_preference_side* chosen, const mlxc_preference_s
     if (pairs < 0) return invalid("pairs must be >= 0");
     if (int rc = check_dtype(dtype, "dtype")) return rc;
     for (const mlxc_preference_side* s : {chosen, rejected}) {
-        if (s->length < 0 || s->length > INT32_MAX) return invalid("length must lie in [0, 2^31)");
+        if (s->length < 0 || s->length >= (int64_t{1} << 30))
+            return invalid("length must lie in [0, 2^30)");
         if (s->length > 0 && pairs > INT64_MAX / 4 / s->length)
             return invalid("pairs * length overflows int64");
         if (values && pairs > 0 && s->length > 0 && !s->values)
