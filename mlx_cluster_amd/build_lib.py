@@ -74,7 +74,7 @@ def build(verbose: bool = False, extra_flags: list[str] | None = None, out: str 
     return out
 
 
-BINDING_SRC = os.path.join(CSRC, "torch_binding.cpp")
+BINDING_SOURCES = [os.path.join(CSRC, f) for f in ("torch_binding.cpp", "torch_training.cpp")]
 
 
 def binding_path() -> str:
@@ -83,7 +83,7 @@ def binding_path() -> str:
 
 
 def build_binding(verbose: bool = False, lib: str = OUT) -> str:
-    """Compiles the compiled fast path (torch_binding.cpp, host code only)
+    """Compiles the compiled fast path (BINDING_SOURCES, host code only)
     against torch's headers and libraries and the in-tree libmlxc.so, with
     hipcc and no source translation step."""
     import sysconfig
@@ -92,13 +92,20 @@ def build_binding(verbose: bool = False, lib: str = OUT) -> str:
     import torch.utils.cpp_extension as ce
     out = binding_path()
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-    cmd = [HIPCC, "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
-           "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
+    flags = ["-O2", "-std=c++17", "-fPIC", "-Wall",
+             "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
            "-DTORCH_EXTENSION_NAME=_mlxc_torch", "-DTORCH_API_INCLUDE_EXTENSION_H",
            "-I", INCLUDE, "-I", sysconfig.get_paths()["include"]]
     for d in ce.include_paths(device_type="cuda"):
-        cmd += ["-isystem", d]
-    cmd += [BINDING_SRC, "-o", out + ".tmp"]
+        flags += ["-isystem", d]
+    from concurrent.futures import ThreadPoolExecutor
+    obj_dir = os.path.join(BUILD_DIR, "binding")
+    os.makedirs(obj_dir, exist_ok=True)
+    objs = [os.path.join(obj_dir, os.path.basename(src) + ".o") for src in BINDING_SOURCES]
+    with ThreadPoolExecutor(len(objs)) as pool:
+        list(pool.map(lambda so: _run([HIPCC, *flags, "-c", so[0], "-o", so[1]], verbose, so[0]),
+                      zip(BINDING_SOURCES, objs)))
+    cmd = [HIPCC, "-shared", "-fPIC", *objs, "-o", out + ".tmp"]
     for d in ce.library_paths(device_type="cuda"):
         cmd += ["-L", d, f"-Wl,-rpath,{d}"]
     cmd += ["-L", os.path.dirname(lib), "-Wl,-rpath,$ORIGIN", "-lmlxc",

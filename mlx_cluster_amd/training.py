@@ -24,7 +24,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from .walks import (_check_stream_arg, _enter_side_stream, _leave_side_stream, _on, _on_cpu,
+from .walks import (_check_stream_arg, _fast, _enter_side_stream, _leave_side_stream, _on, _on_cpu,
                     _on_device, _ptr, _resolve_device, _side_stream, _stream_handle, _workspace)
 
 _FLOATS = {torch.float32: _lib.MLXC_FLOAT32, torch.bfloat16: _lib.MLXC_BFLOAT16,
@@ -110,6 +110,18 @@ def _read_status(word: torch.Tensor, stream, what: str) -> None:
         stream.synchronize()
     _raise_bits = int(word[0].item())
     _raise_bad(_raise_bits, what)
+
+
+def _plain(stream, number, *tensors) -> bool:
+    """Whether the compiled path (csrc/torch_training.cpp) may take a call: it
+    looks at the tensors itself, and leaves what it does not take to the code
+    below."""
+    return (_fast is not None and stream is None and type(number) is float and
+            all(isinstance(t, torch.Tensor) for t in tensors))
+
+
+def _plain_int(x) -> bool:
+    return x is None or (type(x) is int and x > 0)
 
 
 class _Launch:
@@ -217,6 +229,10 @@ def embedding(weight, nodes, *, scale: float = 1.0, sparse_grad: bool = False, c
             stays asynchronous.
         stream: as in random_walk ('cpu' runs the host twin).
     """
+    if _plain(stream, scale, weight, nodes) and not sparse_grad:
+        res = _fast.embedding(weight, nodes, scale, bool(check))
+        if res is not None:
+            return res
     _check_stream_arg(stream)
     weight = _table(weight)
     nodes = _tensor(nodes, _NODES, "nodes")
@@ -288,6 +304,10 @@ def embedding_grad(grad, nodes, num_nodes: int, *, scale: float = 1.0, sparse: b
             the call stays asynchronous with check=False.
         out_dtype: of the gradient (default: grad's).
     """
+    if out_dtype is None and type(num_nodes) is int and _plain(stream, scale, grad, nodes):
+        res = _fast.embedding_grad(grad, nodes, num_nodes, scale, bool(sparse), bool(check))
+        if res is not None:
+            return res
     _check_stream_arg(stream)
     grad = _tensor(grad, _FLOATS, "grad")
     nodes = _tensor(nodes, _NODES, "nodes")
@@ -397,6 +417,10 @@ def window_scores(weight, walks, context_size: Optional[int] = None, *, scale: f
     weight, sparse_grad, check, stream: as in embedding; differentiable in
     weight.  walks: int64 or int32 [N, nodes], context_size in [2, min(32, nodes)].
     """
+    if _plain(stream, scale, weight, walks) and _plain_int(context_size) and not sparse_grad:
+        res = _fast.window_scores(weight, walks, context_size or 0, scale, bool(check))
+        if res is not None:
+            return res
     _check_stream_arg(stream)
     weight = _table(weight)
     walks, C = _walks(walks, context_size)
@@ -418,6 +442,12 @@ def window_scores_grad(grad, weight, walks, context_size: Optional[int] = None, 
     check, stream: as in window_scores.  sparse, out_dtype (default: weight's)
     and the result: as in embedding_grad.
     """
+    if out_dtype is None and _plain_int(context_size) and \
+            _plain(stream, scale, grad, weight, walks):
+        res = _fast.window_scores_grad(grad, weight, walks, context_size or 0, scale, bool(sparse),
+                                       bool(check))
+        if res is not None:
+            return res
     _check_stream_arg(stream)
     weight = _table(weight)
     walks, C = _walks(walks, context_size)
@@ -592,6 +622,16 @@ def preference_loss_grad(chosen, rejected, ref_chosen=None, ref_rejected=None, *
     rewards, and its gradients in the values' shapes and dtype (0 in masked
     places).  Arguments as in preference_loss.
     """
+    if reduction in ("mean", "sum") and type(label_smoothing) is float and \
+            0.0 <= label_smoothing <= 1.0 and _plain(stream, beta, chosen, rejected) and \
+            math.isfinite(beta) and all(t is None or isinstance(t, torch.Tensor) for t in
+                                        (ref_chosen, ref_rejected, chosen_mask, rejected_mask)):
+        res = _fast.preference_loss_grad(
+            chosen, rejected, ref_chosen, ref_rejected, chosen_mask, rejected_mask, beta,
+            label_smoothing, (_lib.MLXC_PREFERENCE_NORMALIZE if normalize else 0) |
+            (_lib.MLXC_PREFERENCE_SUM if reduction == "sum" else 0))
+        if res is not None:
+            return res
     _check_stream_arg(stream)
     sides = _Sides(chosen, rejected, ref_chosen, ref_rejected, chosen_mask, rejected_mask, beta,
                    label_smoothing, normalize, reduction)
