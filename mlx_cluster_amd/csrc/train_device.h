@@ -54,6 +54,22 @@ __device__ __forceinline__ void store_pack(typename E::S* p, const float (&x)[N]
     *reinterpret_cast<Pack<typename E::S, N>*>(p) = k;
 }
 
+// A store past the caches, for what the call does not read again.
+template <typename S, int N>
+__device__ __forceinline__ void stream_pack(S* p, const Pack<S, N>& k) {
+    constexpr int kBytes = sizeof(S) * N;
+    if constexpr (kBytes == 16) {
+        typedef uint32_t Words __attribute__((ext_vector_type(4)));
+        __builtin_nontemporal_store(__builtin_bit_cast(Words, k), reinterpret_cast<Words*>(p));
+    } else if constexpr (kBytes == 8) {
+        __builtin_nontemporal_store(__builtin_bit_cast(uint64_t, k), reinterpret_cast<uint64_t*>(p));
+    } else if constexpr (kBytes == 4) {
+        __builtin_nontemporal_store(__builtin_bit_cast(uint32_t, k), reinterpret_cast<uint32_t*>(p));
+    } else {
+        *p = k.v[0];
+    }
+}
+
 // Nodes of a call: int64 or int32, num_rows of them valid.
 struct Nodes {
     const void* p;

@@ -97,43 +97,60 @@ struct Fragment {
     Pack<typename E::S, Matrix<E>::kPer> v[kSteps];
 };
 
-// Values [from, from + kSteps * kStep) of this lane's row (node, -1: zeros).
-template <typename E, int kSteps>
+// Values [from, from + kSteps * kStep) of this lane's row, zeros from dim on.
+// kAligned: packs of kPer values lie aligned and fill the rows, and the table
+// has a row; without a branch then, and of no node the first row's.  Else
+// zeros of no node.
+template <typename E, int kSteps, bool kAligned>
 __device__ __forceinline__ void load_fragment(Fragment<E, kSteps>& f,
                                               const typename E::S* __restrict__ weight,
                                               int64_t row_stride, int32_t dim, int width,
-                                              int64_t node, int32_t from) {
+                                              int32_t node, int32_t from) {
+    constexpr int kPer = Matrix<E>::kPer;
     const int lane = threadIdx.x % kWave;
     const typename E::S* row = weight + (node < 0 ? 0 : node) * row_stride;
-    const int32_t end = node < 0 ? 0 : dim;
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s)
-        f.v[s] = load_values<E, Matrix<E>::kPer>(
-            row, from + s * Matrix<E>::kStep + lane / kTileRows * Matrix<E>::kPer, end, width);
+    for (int s = 0; s < kSteps; ++s) {
+        const int32_t at = from + s * Matrix<E>::kStep + lane / kTileRows * kPer;
+        if (kAligned) {
+            f.v[s] = *reinterpret_cast<const Pack<typename E::S, kPer>*>(row + (at < dim ? at : 0));
+            if (dim % Matrix<E>::kStep != 0 && at >= dim) {
+#pragma unroll
+                for (int q = 0; q < kPer; ++q) f.v[s].v[q] = 0;
+            }
+        } else {
+            f.v[s] = load_values<E, kPer>(row, at, node < 0 ? 0 : dim, width);
+        }
+    }
 }
 
 // The node of row 16 * t + lane % 16 of a walk, -1 from M on.
-__device__ __forceinline__ int64_t tile_node(const Walks& walks, int64_t n, int64_t t, bool& bad) {
-    const int64_t i = t * kTileRows + threadIdx.x % kTileRows;
-    return i < walks.walk_nodes ? node_at(walks.nodes, n * walks.walk_nodes + i, bad) : -1;
+__device__ __forceinline__ int32_t tile_node(const Walks& walks, int64_t n, int32_t t, bool& bad) {
+    const int64_t i = static_cast<int64_t>(t) * kTileRows + threadIdx.x % kTileRows;
+    return i < walks.walk_nodes
+               ? static_cast<int32_t>(node_at(walks.nodes, n * walks.walk_nodes + i, bad))
+               : -1;
 }
 
 // Scores of the pairs between row tile t (rows) and t + ahead (columns).
 __device__ __forceinline__ void store_scores(const f32x4& acc, const Walks& walks, int64_t n,
-                                             int64_t t, int ahead, uint32_t rows_valid,
+                                             int32_t t, int ahead, uint32_t rows_valid,
                                              uint32_t cols_valid, float scale,
                                              float* __restrict__ scores) {
     const int lane = threadIdx.x % kWave;
-    const int64_t W = walks.windows();
-    const int c = lane % kTileRows;
+    const int32_t W = static_cast<int32_t>(walks.windows());
+    const int c = lane % kTileRows, r0 = lane / kTileRows * 4;
+    // entry (j, k) is at (n * W + j) * (C - 1) + k - 1: from one row to the
+    // next of the lane's column k falls by one
+    float* first = scores + (n * W + t * kTileRows + r0) * (walks.ctx - 1) +
+                   (ahead * kTileRows + c - r0 - 1);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-        const int r = lane / kTileRows * 4 + q;
-        const int64_t j = t * kTileRows + r;
+        const int r = r0 + q;
         const int k = ahead * kTileRows + c - r;
-        if (j >= W || k < 1 || k >= walks.ctx) continue;
+        if (t * kTileRows + r >= W || k < 1 || k >= walks.ctx) continue;
         const bool both = (rows_valid >> r) & (cols_valid >> c) & 1;
-        scores[(n * W + j) * (walks.ctx - 1) + k - 1] = both ? acc[q] * scale : 0.f;
+        first[static_cast<int64_t>(q) * (walks.ctx - 2)] = both ? acc[q] * scale : 0.f;
     }
 }
 
@@ -147,33 +164,33 @@ struct Split {
 // the kAhead tiles after it, which are all that C - 1 <= 16 * kAhead places
 // reach, kept in registers until they are rows themselves; the next tile's
 // loads fly meanwhile.  dim <= kSteps * kStep.
-template <typename E, int kSteps, int kAhead>
+template <typename E, int kSteps, int kAhead, bool kAligned>
 __global__ __launch_bounds__(kBlock) void window_scores_kernel(
     const typename E::S* __restrict__ weight, int64_t row_stride, int32_t dim, int width,
     Walks walks, Split split, float scale, float* __restrict__ scores, int64_t* status) {
-    const int64_t W = walks.windows();
-    const int64_t row_tiles = (W + kTileRows - 1) / kTileRows;
+    const int32_t row_tiles = static_cast<int32_t>((walks.windows() + kTileRows - 1) / kTileRows);
     bool bad = false;
     for (int64_t u = blockIdx.x * static_cast<int64_t>(kWaves) + threadIdx.x / kWave;
          u < walks.num_walks * split.parts; u += static_cast<int64_t>(gridDim.x) * kWaves) {
         const int64_t n = u / split.parts;
-        const int64_t first = (u - n * split.parts) * split.per;
-        const int64_t last = first + split.per < row_tiles ? first + split.per : row_tiles;
+        const int32_t first = static_cast<int32_t>(u - n * split.parts) * split.per;
+        const int32_t last = row_tiles - first > split.per ? first + split.per : row_tiles;
         Fragment<E, kSteps> f[kAhead + 1];
         uint32_t valid[kAhead + 1];
 #pragma unroll
         for (int a = 0; a <= kAhead; ++a) {
-            const int64_t node = tile_node(walks, n, first + a, bad);
+            const int32_t node = tile_node(walks, n, first + a, bad);
             valid[a] = static_cast<uint32_t>(__ballot(node >= 0)) & 0xffffu;
-            load_fragment<E, kSteps>(f[a], weight, row_stride, dim, width, node, 0);
+            load_fragment<E, kSteps, kAligned>(f[a], weight, row_stride, dim, width, node, 0);
         }
-        int64_t next_node = tile_node(walks, n, first + kAhead + 1, bad);
-        for (int64_t t = first; t < last; ++t) {
+        int32_t next_node = tile_node(walks, n, first + kAhead + 1, bad);
+        for (int32_t t = first; t < last; ++t) {
             Fragment<E, kSteps> next;
             uint32_t next_valid = 0;
             if (t + 1 < last) {
                 next_valid = static_cast<uint32_t>(__ballot(next_node >= 0)) & 0xffffu;
-                load_fragment<E, kSteps>(next, weight, row_stride, dim, width, next_node, 0);
+                load_fragment<E, kSteps, kAligned>(next, weight, row_stride, dim, width, next_node,
+                                                   0);
                 next_node = tile_node(walks, n, t + kAhead + 2, bad);
             }
 #pragma unroll
@@ -199,20 +216,19 @@ __global__ __launch_bounds__(kBlock) void window_scores_kernel(
 // Rows of any length: for every row tile, kSteps steps of all its tiles at a
 // time.  A tile's rows are loaded again for the kAhead row tiles before it, as
 // a rule from the caches.
-template <typename E, int kSteps, int kAhead>
+template <typename E, int kSteps, int kAhead, bool kAligned>
 __global__ __launch_bounds__(kBlock) void window_scores_long_kernel(
     const typename E::S* __restrict__ weight, int64_t row_stride, int32_t dim, int width,
     Walks walks, Split split, float scale, float* __restrict__ scores, int64_t* status) {
-    const int64_t W = walks.windows();
-    const int64_t row_tiles = (W + kTileRows - 1) / kTileRows;
+    const int32_t row_tiles = static_cast<int32_t>((walks.windows() + kTileRows - 1) / kTileRows);
     bool bad = false;
     for (int64_t u = blockIdx.x * static_cast<int64_t>(kWaves) + threadIdx.x / kWave;
          u < walks.num_walks * split.parts; u += static_cast<int64_t>(gridDim.x) * kWaves) {
         const int64_t n = u / split.parts;
-        const int64_t first = (u - n * split.parts) * split.per;
-        const int64_t last = first + split.per < row_tiles ? first + split.per : row_tiles;
-        for (int64_t t = first; t < last; ++t) {
-            int64_t node[kAhead + 1];
+        const int32_t first = static_cast<int32_t>(u - n * split.parts) * split.per;
+        const int32_t last = row_tiles - first > split.per ? first + split.per : row_tiles;
+        for (int32_t t = first; t < last; ++t) {
+            int32_t node[kAhead + 1];
             f32x4 acc[kAhead + 1];
 #pragma unroll
             for (int a = 0; a <= kAhead; ++a) {
@@ -223,7 +239,8 @@ __global__ __launch_bounds__(kBlock) void window_scores_long_kernel(
                 Fragment<E, kSteps> f[kAhead + 1];
 #pragma unroll
                 for (int a = 0; a <= kAhead; ++a)
-                    load_fragment<E, kSteps>(f[a], weight, row_stride, dim, width, node[a], from);
+                    load_fragment<E, kSteps, kAligned>(f[a], weight, row_stride, dim, width,
+                                                       node[a], from);
 #pragma unroll
                 for (int a = 0; a <= kAhead; ++a)
 #pragma unroll
@@ -254,7 +271,7 @@ __device__ __forceinline__ float band_entry(const float* __restrict__ grad, cons
 
 // A tile's gradients without the matrix unit: only the band's own products.
 template <typename E>
-__device__ __noinline__ void band_rows(const float* __restrict__ grad,
+__device__ __forceinline__ void band_rows(const float* __restrict__ grad,
                                        const typename E::S* __restrict__ weight, int64_t row_stride,
                                        int32_t dim, const Walks& walks, int64_t n, int64_t i0,
                                        int32_t col0, int32_t cols, float* __restrict__ rows) {
@@ -281,114 +298,139 @@ __device__ __noinline__ void band_rows(const float* __restrict__ grad,
 // One wavefront: 16 places of a walk, 16 * kPer columns.  The band's entries
 // are the first operand, loaded where a lane needs them (lane % 16 the place,
 // lane / 16 one of the four other places of a step); the rows the second: lane
-// (k, c) holds values c * kPer + 0 .. kPer - 1 of place k, so that instruction
-// q's columns are the values of index q of every pack, and a lane's results are
-// kPer consecutive values of four places again.  In float32 throughout: a
-// 16-bit band would round the scores' gradients.
+// (k, c) holds values 4 c .. 4 c + 3 of place k (and of 16-bit rows 64 + those),
+// so that instruction q's columns are the values of index q of every pack, and a
+// lane's results are four consecutive values of four places again: stores of
+// whole lines.  In float32 throughout: a 16-bit band would round the scores'
+// gradients.
 //
 // Zeros outside the band meet every row of the step, and 0 * inf is NaN: where
 // a result is not finite, the tile is done again by the band's products alone.
 //
-// kAligned: packs of kPer values lie aligned and fill the rows.  Places without
-// a node, and columns past the last, then load the table's first row and
-// values, without a branch: their entries are 0, or their results not stored.
-template <typename E, bool kAligned>
+// kRow says how rows are loaded: kWhole, in aligned packs, and dim is a multiple
+// of the block's columns; kAligned, in aligned packs that fill the rows;
+// kMasked, any.  The first two load without a branch: of places without a node
+// the table's first row, of columns past the last the first; their entries are
+// 0, or their results not stored.
+//
+// Bound by the stores (five sixths of what it moves) with the vector units half
+// busy beside them: 65,536 walks of 81 nodes, 128 bfloat16, context 10, 4.1 GB in
+// 1,050 us (a copy of as many bytes: 850).  One place a wavefront and one column a lane took 15,600.
+enum class RowLoad { kWhole, kAligned, kMasked };
+
+template <typename E, RowLoad kRow, bool kStreamed>
 __global__ __launch_bounds__(kBlock) void window_rows_grad_kernel(
     const float* __restrict__ grad, const typename E::S* __restrict__ weight, int64_t row_stride,
     int32_t dim, int width, Walks walks, int64_t tiles, float* __restrict__ rows) {
     constexpr int kPer = Matrix<E>::kPer;
     constexpr int kCols = kTileRows * kPer;
-    constexpr int kAhead = 4;  // steps of four places whose loads fly together
+    constexpr int kParts = kPer / 4;  // packs of four values
+    constexpr int kAhead = 2;         // steps of four places whose loads fly together (4: 1,090 us)
     const int lane = threadIdx.x % kWave;
     const int part = lane / kTileRows, c = lane % kTileRows;
     const int32_t M = walks.walk_nodes, C = walks.ctx;
     const int32_t reach = C - 1;
     const int32_t W = static_cast<int32_t>(walks.windows());
-    const int32_t col0 = blockIdx.y * kCols, col = col0 + c * kPer;
+    const int32_t col0 = blockIdx.y * kCols;
+    int32_t col[kParts];
+#pragma unroll
+    for (int h = 0; h < kParts; ++h) col[h] = col0 + h * 4 * kTileRows + c * 4;
     struct Steps {
-        Pack<typename E::S, kPer> x[kAhead];
+        Pack<typename E::S, 4> x[kAhead][kParts];
         float a[kAhead];
     };
     for (int64_t u = blockIdx.x * static_cast<int64_t>(kWaves) + threadIdx.x / kWave;
          u < walks.num_walks * tiles; u += static_cast<int64_t>(gridDim.x) * kWaves) {
         const int64_t n = u / tiles;
         const int32_t i0 = static_cast<int32_t>(u - n * tiles) * kTileRows;
-        const int32_t from = i0 > reach ? (i0 - reach) / 4 * 4 : 0;
-        const int32_t to = M - i0 > kTileRows + reach ? i0 + kTileRows + reach : M;
-        // the nodes of places [from, from + 128), two a lane (16 + 2 * 31 + 3
-        // places at most)
-        int32_t node[2];
+        // places [from, to) meet the tile's: 16 + 2 * 31 + 3 at most
+        const int32_t from = __builtin_amdgcn_readfirstlane(i0 > reach ? (i0 - reach) / 4 * 4 : 0);
+        const int32_t span = __builtin_amdgcn_readfirstlane(
+            (M - i0 > kTileRows + reach ? i0 + kTileRows + reach : M) - from);
+        int32_t node[2];  // of places from + lane, from + 64 + lane
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             bool bad = false;
-            const int32_t o = from + h * kWave + lane;
-            node[h] = o < to ? static_cast<int32_t>(node_at(walks.nodes, n * M + o, bad)) : -1;
+            const int32_t o = h * kWave + lane;
+            node[h] = o < span
+                          ? static_cast<int32_t>(node_at(walks.nodes, n * M + from + o, bad))
+                          : -1;
         }
-        const auto node_of = [&](int32_t o) {  // by all lanes; o in [from, from + 128)
-            const int32_t at = o - from;
-            const int32_t near = __shfl(node[0], at & (kWave - 1), kWave);
-            const int32_t far = __shfl(node[1], at & (kWave - 1), kWave);
-            return at < kWave ? near : far;
+        // by all lanes: of place from + o, o < 128
+        const auto node_of = [&](int32_t o) {
+            const int32_t near = __shfl(node[0], o & (kWave - 1), kWave);
+            const int32_t far = __shfl(node[1], o & (kWave - 1), kWave);
+            return o < kWave ? near : far;
         };
-        const int32_t i = i0 + c;  // the lane's place in the first operand
+        // places from here on as their distance to `from`
+        const int32_t i = i0 - from + c;  // the lane's in the first operand
+        const int32_t w = W - from;       // windows start before this one
         const bool own = node_of(i) >= 0;
-        const float* band = grad + n * W * (C - 1) - 1;
+        // entry (j, j + k) of the band is at band[j * (C - 1) + k]
+        const float* band = grad + (n * W + from) * (C - 1) - 1;
         const auto load = [&](Steps& s, int32_t o0) {
 #pragma unroll
             for (int q = 0; q < kAhead; ++q) {
                 const int32_t o = o0 + 4 * q + part;
-                const int32_t v = node_of(o);  // -1 from `to` on
+                const int32_t v = node_of(o);  // -1 from `span` on
                 const int32_t j = i < o ? i : o, k = i < o ? o - i : i - o;
-                const bool pair = own && v >= 0 && k >= 1 && k < C && j < W;
-                s.a[q] = pair ? band[static_cast<int64_t>(j) * (C - 1) + k] : 0.f;
+                const bool pair = own && v >= 0 && k >= 1 && k < C && j < w;
+                s.a[q] = pair ? band[static_cast<uint32_t>(j * (C - 1) + k)] : 0.f;
                 const typename E::S* row = weight + static_cast<int64_t>(v < 0 ? 0 : v) * row_stride;
-                if (kAligned)
-                    s.x[q] = *reinterpret_cast<const Pack<typename E::S, kPer>*>(
-                        row + (col < dim ? col : 0));
-                else
-                    s.x[q] = load_values<E, kPer>(row, col, v < 0 ? 0 : dim, width);
+#pragma unroll
+                for (int h = 0; h < kParts; ++h)
+                    if (kRow == RowLoad::kMasked)
+                        s.x[q][h] = load_values<E, 4>(row, col[h], v < 0 ? 0 : dim, width);
+                    else
+                        s.x[q][h] = *reinterpret_cast<const Pack<typename E::S, 4>*>(
+                            row + (kRow == RowLoad::kWhole || col[h] < dim ? col[h] : 0));
             }
         };
         f32x4 acc[kPer];
 #pragma unroll
         for (int q = 0; q < kPer; ++q) acc[q] = f32x4{0.f, 0.f, 0.f, 0.f};
         Steps s;
-        load(s, from);
-        for (int32_t o0 = from; o0 < to; o0 += 4 * kAhead) {
+        load(s, 0);
+        for (int32_t o0 = 0; o0 < span; o0 += 4 * kAhead) {
             Steps next;
-            if (o0 + 4 * kAhead < to) load(next, o0 + 4 * kAhead);
+            if (o0 + 4 * kAhead < span) load(next, o0 + 4 * kAhead);
 #pragma unroll
             for (int q = 0; q < kAhead; ++q)
 #pragma unroll
                 for (int e = 0; e < kPer; ++e)
-                    acc[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(s.a[q], E::load(s.x[q].v[e]),
-                                                                  acc[e], 0, 0, 0);
+                    acc[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                        s.a[q], E::load(s.x[q][e / 4].v[e % 4]), acc[e], 0, 0, 0);
             s = next;
         }
         float odd = 0.f;  // NaN if a result is not finite
 #pragma unroll
         for (int q = 0; q < kPer; ++q)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) odd += acc[q][r] * 0.f;
+            for (int r = 0; r < 4; ++r) odd = __builtin_fmaf(acc[q][r], 0.f, odd);
         if (__ballot(odd != 0.f)) {
             band_rows<E>(grad, weight, row_stride, dim, walks, n, i0, col0, kCols, rows);
             continue;
         }
+        float* first = rows + (n * M + i0 + part * 4) * dim;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int32_t place = i0 + part * 4 + r;
-            if (place >= M) continue;
-            float* to_row = rows + (n * M + place) * dim + col;
-            if (kAligned || dim % 4 == 0) {
+            if (i0 + part * 4 + r >= M) continue;
 #pragma unroll
-                for (int q = 0; q < kPer; q += 4)
-                    if (col + q < dim)
-                        *reinterpret_cast<f32x4*>(to_row + q) =
-                            f32x4{acc[q][r], acc[q + 1][r], acc[q + 2][r], acc[q + 3][r]};
-            } else {
+            for (int h = 0; h < kParts; ++h) {
+                float* to = first + r * dim + col[h];
+                if (kRow != RowLoad::kMasked || dim % 4 == 0) {
+                    const f32x4 x = {acc[4 * h][r], acc[4 * h + 1][r], acc[4 * h + 2][r],
+                                     acc[4 * h + 3][r]};
+                    if (kRow != RowLoad::kWhole && col[h] >= dim) continue;
+                    if constexpr (kStreamed)
+                        __builtin_nontemporal_store(x, reinterpret_cast<f32x4*>(to));
+                    else
+                        *reinterpret_cast<f32x4*>(to) = x;
+                } else {
 #pragma unroll
-                for (int q = 0; q < kPer; ++q)
-                    if (col + q < dim) to_row[q] = acc[q][r];
+                    for (int q = 0; q < 4; ++q)
+                        if (col[h] + q < dim) to[q] = acc[4 * h + q][r];
+                }
             }
         }
     }
@@ -431,11 +473,15 @@ int scores_launch(const Table& table, const Walks& walks, float scale, float* sc
     unsigned grid;
     if (int rc = split_walks(walks, split)) return rc;
     if (int rc = wave_grid(walks.num_walks * split.parts, grid)) return rc;
-    auto* kernel = kLong ? window_scores_long_kernel<E, kSteps, kAhead>
-                         : window_scores_kernel<E, kSteps, kAhead>;
+    const int width = table_width<E>(table);
+    const bool aligned = width == Matrix<E>::kPer && table.num_rows > 0;
+    auto* kernel = kLong ? aligned ? window_scores_long_kernel<E, kSteps, kAhead, true>
+                                   : window_scores_long_kernel<E, kSteps, kAhead, false>
+                   : aligned ? window_scores_kernel<E, kSteps, kAhead, true>
+                             : window_scores_kernel<E, kSteps, kAhead, false>;
     hipLaunchKernelGGL(kernel, dim3(grid), dim3(kBlock), 0, stream,
                        static_cast<const typename E::S*>(table.p), table.row_stride, table.dim,
-                       table_width<E>(table), walks, split, scale, scores, status);
+                       width, walks, split, scale, scores, status);
     MLXC_HIP_TRY(hipGetLastError());
     return MLXC_OK;
 }
@@ -472,8 +518,18 @@ int rows_grad_typed(const float* grad, const Table& table, const Walks& walks, f
     unsigned grid;
     if (int rc = wave_grid(walks.num_walks * tiles, grid)) return rc;
     const int width = table_width<E>(table);
-    auto* kernel = width == Matrix<E>::kPer ? window_rows_grad_kernel<E, true>
-                                            : window_rows_grad_kernel<E, false>;
+    // Rows that the caches cannot hold until they are added up are streamed past
+    // them: 5.3 M rows of 128 1,085 -> 1,043 us, and their sums 633 -> 607 (377,000 of 100,
+    // 151 MB: 102 -> 89, but the sums 47 -> 63).
+    const bool streamed = static_cast<size_t>(walks.count()) * table.dim * sizeof(float) >
+                          (size_t{256} << 20);
+    const bool whole = table.dim % cols == 0;
+    auto* kernel =
+        width < 4 ? window_rows_grad_kernel<E, RowLoad::kMasked, false>
+        : whole   ? streamed ? window_rows_grad_kernel<E, RowLoad::kWhole, true>
+                             : window_rows_grad_kernel<E, RowLoad::kWhole, false>
+        : streamed ? window_rows_grad_kernel<E, RowLoad::kAligned, true>
+                   : window_rows_grad_kernel<E, RowLoad::kAligned, false>;
     hipLaunchKernelGGL(kernel, dim3(grid, (table.dim + cols - 1) / cols),
                        dim3(kBlock), 0, stream, grad, static_cast<const typename E::S*>(table.p),
                        table.row_stride, table.dim, width, walks, tiles, rows);
