@@ -15,7 +15,8 @@ REPO_DIR = os.path.dirname(PKG_DIR)
 CSRC = os.path.join(PKG_DIR, "csrc")
 SOURCES = [os.path.join(CSRC, f) for f in
            ("mlxc_api.hip", "prep_kernels.hip", "uniform_walk.hip", "node2vec_walk.hip",
-            "csr_build.hip", "windows.hip", "gather_probe.hip", "train_api.hip", "embedding.hip",
+            "csr_build.hip", "windows.hip", "gather_probe.hip", "train_api.hip", "place_sort.hip",
+            "embedding.hip",
             "window_scores.hip", "preference.hip", "host_walk.cpp", "host_csr.cpp",
             "host_train.cpp")]
 OUT = os.path.join(PKG_DIR, "libmlxc.so")

@@ -4,15 +4,16 @@
 //   lookup     y[i, :] = s * W[x_i, :]
 //   gradient   G[v, :] = s * sum over i with x_i = v of g[i, :]
 //
-// The gradient sorts (node, place) by node, stable, with an LSD radix sort of
-// the bits that a node can have, so that a node's places stand together in
-// ascending order; then every row adds its places up.  Places without a node
-// are dropped by the first pass.  Walks visit hubs tens of thousands of times,
-// so the sorted places are added up in tiles of 32, each by one group of lanes
-// whatever runs it holds; a run that crosses tiles is put together from its
-// tiles' parts, a hub's from sums of 16 tiles, of 16 of these, and so on.  So no
-// lane adds more than a few dozen rows, nothing is added with atomics, and the
-// order of a sum depends on the places alone.
+// The gradient sorts the places by node (place_sort.hip).  Walks visit hubs tens
+// of thousands of times, so the sorted places are added up in tiles of 32, each
+// by one group of lanes whatever runs it holds; a run that crosses tiles is put
+// together from its tiles' parts, a hub's from sums of 16 tiles, of 16 of these,
+// and so on.  So no lane adds more than a few dozen rows, nothing is added with
+// atomics, and the order of a sum depends on the places alone.
+//
+// Bound by the gather of the rows and the table's stores.  2.65 M rows of 128
+// bfloat16 into a table of 2^20: @GWUS@.  One wavefront a node, place after
+// place, took 1,530 us for the sums alone.
 #include "train_host.h"
 
 namespace mlxc {
@@ -72,233 +73,15 @@ __global__ __launch_bounds__(kBlock) void embedding_kernel(
     report_bad(bad, status);
 }
 
-// ------------------------------------------------------------- sort by node
-
-constexpr int kDigitBits = 8;
-constexpr int kDigits = 1 << kDigitBits;
-constexpr int kItems = 16;               // keys a thread
-constexpr int kTile = kBlock * kItems;   // keys a block
-constexpr int kWaves = kBlock / kWave;
-constexpr int kWaveTile = kWave * kItems;
-static_assert(kDigits == kBlock, "one digit a thread");
-
-constexpr int kWordStatus = 0;  // of the workspace header
-
-// Exclusive prefix of one value a thread over the block; *total the sum.  `tot`
-// is kWaves words of LDS.  Contains two barriers.
-__device__ __forceinline__ uint32_t block_prefix(uint32_t v, uint32_t* tot, uint32_t* total) {
-    const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave;
-    uint32_t inc = v;
-#pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) {
-        const uint32_t u = __shfl_up(inc, o, kWave);
-        if (lane >= o) inc += u;
-    }
-    if (lane == kWave - 1) tot[w] = inc;
-    __syncthreads();
-    uint32_t before = 0, all = 0;
-    for (int k = 0; k < kWaves; ++k) {
-        if (k < w) before += tot[k];
-        all += tot[k];
-    }
-    *total = all;
-    __syncthreads();
-    return before + inc - v;
-}
-
-// Lanes of the wavefront that are active and hold this lane's digit.
-__device__ __forceinline__ uint64_t same_digit(uint32_t d, bool active) {
-    uint64_t peers = __ballot(active);
-#pragma unroll
-    for (int b = 0; b < kDigitBits; ++b) {
-        const bool bit = (d >> b) & 1;
-        const uint64_t set = __ballot(bit);
-        peers &= bit ? set : ~set;
-    }
-    return peers;
-}
-
-// The keys of a pass: the call's nodes (places are their indices, count of
-// them), or the last pass's, *valid of them.
-struct SortIn {
-    Nodes nodes;
-    int64_t count;
-    const uint32_t* keys;
-    const uint32_t* places;
-    const uint32_t* valid;
-};
-
-// counts[d * tiles + tile] <- the tile's keys of digit d.  The first pass also
-// checks the nodes, and zeroes the words that later kernels need zeroed.
-template <bool kFirst>
-__global__ __launch_bounds__(kBlock) void digit_count_kernel(SortIn in, int shift, uint32_t tiles,
-                                                             uint32_t* __restrict__ counts,
-                                                             uint32_t* __restrict__ zero,
-                                                             int64_t zero_words,
-                                                             int64_t* __restrict__ work) {
-    __shared__ uint32_t cnt[kDigits];
-    const int t = threadIdx.x;
-    cnt[t] = 0;
-    __syncthreads();
-    const int64_t n = kFirst ? in.count : static_cast<int64_t>(*in.valid);
-    const int64_t base = static_cast<int64_t>(blockIdx.x) * kTile;
-    bool bad = false;
-#pragma unroll
-    for (int s = 0; s < kItems; ++s) {
-        const int64_t i = base + s * kBlock + t;
-        if (i >= n) break;
-        const int64_t key = kFirst ? node_at(in.nodes, i, bad) : static_cast<int64_t>(in.keys[i]);
-        if (key >= 0) atomicAdd(&cnt[(static_cast<uint32_t>(key) >> shift) & (kDigits - 1)], 1u);
-    }
-    __syncthreads();
-    counts[static_cast<size_t>(t) * tiles + blockIdx.x] = cnt[t];
-    if (kFirst) {
-        for (int64_t k = blockIdx.x * static_cast<int64_t>(kBlock) + t; k < zero_words;
-             k += static_cast<int64_t>(gridDim.x) * kBlock)
-            zero[k] = 0;
-        report_bad(bad, work + kWordStatus);
-    }
-}
-
-// Exclusive prefix over each digit's tiles, in place, one block a digit;
-// totals[digit] <- the sum.
-__global__ __launch_bounds__(kBlock) void digit_prefix_kernel(uint32_t* __restrict__ counts,
-                                                              uint32_t tiles,
-                                                              uint32_t* __restrict__ totals) {
-    __shared__ uint32_t tot[kWaves];
-    uint32_t* row = counts + static_cast<size_t>(blockIdx.x) * tiles;
-    uint32_t carry = 0;
-    for (uint32_t base = 0; base < tiles; base += kBlock) {
-        const uint32_t j = base + threadIdx.x;
-        const uint32_t v = j < tiles ? row[j] : 0;
-        uint32_t all;
-        const uint32_t ex = block_prefix(v, tot, &all);
-        if (j < tiles) row[j] = carry + ex;
-        carry += all;
-    }
-    if (threadIdx.x == 0) totals[blockIdx.x] = carry;
-}
-
-// Stable: a key's output place is the keys of lower digits, those of its digit
-// in earlier tiles, and those before it in its tile (wavefront, slot, lane).
-template <bool kFirst>
-__global__ __launch_bounds__(kBlock) void digit_scatter_kernel(
-    SortIn in, int shift, uint32_t tiles, const uint32_t* __restrict__ counts,
-    const uint32_t* __restrict__ totals, uint32_t* __restrict__ keys_out,
-    uint32_t* __restrict__ places_out, uint32_t* __restrict__ valid_out) {
-    __shared__ uint32_t cnt[kWaves][kDigits];
-    __shared__ uint32_t tot[kWaves];
-    const int t = threadIdx.x, w = t / kWave, lane = t % kWave;
-    for (int k = 0; k < kWaves; ++k) cnt[k][t] = 0;
-    uint32_t all;
-    const uint32_t digit_base = block_prefix(totals[t], tot, &all);
-    if (kFirst && blockIdx.x == 0 && t == 0) *valid_out = all;
-    const uint32_t tile_base = counts[static_cast<size_t>(t) * tiles + blockIdx.x];
-    const int64_t n = kFirst ? in.count : static_cast<int64_t>(*in.valid);
-    const int64_t base = static_cast<int64_t>(blockIdx.x) * kTile + w * kWaveTile + lane;
-    uint32_t key[kItems], place[kItems], rank[kItems];
-    uint32_t have = 0;
-#pragma unroll
-    for (int s = 0; s < kItems; ++s) {
-        const int64_t i = base + s * kWave;
-        bool ok = i < n;
-        key[s] = place[s] = 0;
-        if (ok) {
-            if (kFirst) {
-                bool bad = false;
-                const int64_t v = node_at(in.nodes, i, bad);
-                ok = v >= 0;
-                key[s] = static_cast<uint32_t>(v);
-                place[s] = static_cast<uint32_t>(i);
-            } else {
-                key[s] = in.keys[i];
-                place[s] = in.places[i];
-            }
-        }
-        have |= static_cast<uint32_t>(ok) << s;
-    }
-#pragma unroll
-    for (int s = 0; s < kItems; ++s) {
-        const bool ok = (have >> s) & 1;
-        const uint32_t d = (key[s] >> shift) & (kDigits - 1);
-        const uint64_t peers = same_digit(d, ok);
-        const uint32_t before = cnt[w][d];
-        const int r = lane_rank(peers);
-        rank[s] = before + r;
-        // the first of the peers writes after all of them have read (one
-        // wavefront: in order)
-        if (ok && r == 0) cnt[w][d] = before + __popcll(peers);
-        __builtin_amdgcn_wave_barrier();
-    }
-    __syncthreads();
-    uint32_t at = digit_base + tile_base;
-#pragma unroll
-    for (int k = 0; k < kWaves; ++k) {
-        const uint32_t c = cnt[k][t];
-        cnt[k][t] = at;
-        at += c;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int s = 0; s < kItems; ++s) {
-        if (!((have >> s) & 1)) continue;
-        const uint32_t to = cnt[w][(key[s] >> shift) & (kDigits - 1)] + rank[s];
-        keys_out[to] = key[s];
-        places_out[to] = place[s];
-    }
-}
-
-// ------------------------------------------------------------- runs
+// ------------------------------------------------------------- sums
 
 // The sorted places are added up in tiles of kSpan.  Level 1's tiles hold kFan
 // of these, level l's kFan^l.
-constexpr int kSpan = 32;
 constexpr int kFan = 16;
 constexpr int kMaxLevels = 6;
-
-// Coalesced: heads[chunk] <- the runs that start in a chunk of kTile places.
-__global__ __launch_bounds__(kBlock) void count_heads_kernel(const uint32_t* __restrict__ keys,
-                                                             const uint32_t* __restrict__ valid,
-                                                             uint32_t* __restrict__ heads) {
-    __shared__ uint32_t tot[kWaves];
-    const int64_t n = *valid, base = static_cast<int64_t>(blockIdx.x) * kTile;
-    uint32_t c = 0;
-    for (int s = 0; s < kItems; ++s) {
-        const int64_t i = base + s * kBlock + threadIdx.x;
-        c += i < n && (i == 0 || keys[i - 1] != keys[i]);
-    }
-    uint32_t all;
-    block_prefix(c, tot, &all);
-    if (threadIdx.x == 0) heads[blockIdx.x] = all;
-}
-
-// ... then the runs' nodes, and ranks[p] <- the runs that start before tile p
-// of kSpan places.
-__global__ __launch_bounds__(kBlock) void list_runs_kernel(const uint32_t* __restrict__ keys,
-                                                           const uint32_t* __restrict__ valid,
-                                                           const uint32_t* __restrict__ heads,
-                                                           uint32_t* __restrict__ ranks,
-                                                           int64_t* __restrict__ ids) {
-    __shared__ uint32_t tot[kWaves];
-    const int64_t n = *valid, base = static_cast<int64_t>(blockIdx.x) * kTile;
-    uint32_t part = 0, before;
-    for (uint32_t k = threadIdx.x; k < blockIdx.x; k += kBlock) part += heads[k];
-    block_prefix(part, tot, &before);
-    const int64_t first = base + static_cast<int64_t>(threadIdx.x) * kItems;
-    uint32_t is_head = 0;
-    for (int s = 0; s < kItems; ++s) {
-        const int64_t i = first + s;
-        if (i < n && (i == 0 || keys[i - 1] != keys[i])) is_head |= 1u << s;
-    }
-    uint32_t all;
-    uint32_t u = before + block_prefix(__popc(is_head), tot, &all);
-    static_assert(kSpan % kItems == 0, "a tile starts with a thread's places");
-    if (first % kSpan == 0 && first < n) ranks[first / kSpan] = u;
-    for (int s = 0; s < kItems; ++s)
-        if ((is_head >> s) & 1) ids[u++] = keys[first + s];
-}
-
-// ------------------------------------------------------------- sums
+// A level is built where it has this many tiles: with fewer a run has few parts
+// of the level below.
+constexpr int64_t kLevelTiles = 32;
 
 // The lanes that serve one row: 2^lanes_log of them, a pack of N columns each,
 // from column first_column on.
@@ -311,10 +94,7 @@ struct RowShape {
 // past the end of the last row again, and added as zeros: added behind a branch,
 // they are moved there by the compiler, one load after the other (a batch then
 // takes 12.7 us instead of 2).
-#ifndef MLXC_SUM_BATCH
-#define MLXC_SUM_BATCH 8
-#endif
-constexpr int kBatch = MLXC_SUM_BATCH;
+constexpr int kBatch = 8;
 template <typename E, int N, typename Index>
 __device__ __forceinline__ void add_rows(float (&acc)[N], const typename E::S* __restrict__ rows,
                                          int32_t dim, int32_t col, int64_t from, int64_t to,
@@ -468,38 +248,21 @@ struct TileSums {
     int32_t levels;
 };
 
-constexpr int kZeroBlocks = 16;  // a compute unit, of the blocks that write zeros
-
-// What span_sum_kernel left.  The first `finish` blocks put the runs that cross
-// tiles together, each by the group of the tile in which it starts: neighbouring
-// nodes, and those a power of two apart, are often hubs together, and a group a
-// row adds up one hub after the other (2^20 rows of 128 bfloat16: 153 us; so
-// @ROWUS@).  The others write zeros where a row has no run (and its id, -1, if
-// the call lists ids).
+// Puts the runs that cross tiles together, each by the group of the tile in
+// which it starts: neighbouring nodes, and those a power of two apart, are often
+// hubs together, and a group a row would add up one hub after the other.
 template <typename O, int N>
-__global__ __launch_bounds__(kBlock) void row_sum_kernel(
+__global__ __launch_bounds__(kBlock) void run_sum_kernel(
     const uint32_t* __restrict__ keys, const uint32_t* __restrict__ valid,
     const uint32_t* __restrict__ ranks, const uint2* __restrict__ runs, Parts parts, TileSums tiles,
-    RowShape shape, unsigned finish, int64_t num_out, float scale, int64_t* __restrict__ ids,
-    typename O::S* __restrict__ out) {
+    RowShape shape, float scale, typename O::S* __restrict__ out) {
     const int lane = threadIdx.x & ((1 << shape.lanes_log) - 1);
     const int64_t per = kBlock >> shape.lanes_log;  // groups a block
     const int64_t own = threadIdx.x >> shape.lanes_log;
     const int32_t col = ((blockIdx.y << shape.lanes_log) + lane) * N;
-    if (blockIdx.x >= finish) {
-        const int64_t groups = (gridDim.x - finish) * per;
-        for (int64_t v = (blockIdx.x - finish) * per + own; v < num_out; v += groups) {
-            const uint2 run = runs[v];
-            if (run.x != run.y) continue;
-            if (ids && lane == 0 && blockIdx.y == 0) ids[v] = -1;
-            const float zeros[N] = {};
-            if (col < shape.dim) store_pack<O, N>(out + v * shape.dim + col, zeros);
-        }
-        return;
-    }
     if (col >= shape.dim) return;
     const int64_t n = *valid;
-    for (int64_t p = blockIdx.x * per + own; (p + 1) * kSpan < n; p += finish * per) {
+    for (int64_t p = blockIdx.x * per + own; (p + 1) * kSpan < n; p += gridDim.x * per) {
         const uint32_t node = keys[(p + 1) * kSpan - 1];
         const bool leaves = keys[(p + 1) * kSpan] == node;
         const bool entered = p > 0 && keys[p * kSpan - 1] == node;
@@ -541,46 +304,28 @@ __global__ void clear_words_kernel(int64_t* words, int n) {
 
 size_t round256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
 
-int bits_below(int64_t n) {  // bits of n - 1
-    int b = 0;
-    for (uint64_t x = n > 1 ? static_cast<uint64_t>(n - 1) : 0; x; x >>= 1) ++b;
-    return b;
-}
-
+// The workspace: the header, the sort's part, then the sums'.
 struct GradLayout {
-    int passes = 1;
-    uint32_t tiles = 0;
-    size_t keys[2], places[2], counts, totals, valid, runs, heads, ranks, first, last;
-    size_t sums[kMaxLevels], bytes;
+    size_t sort, runs, first, last, sums[kMaxLevels], bytes;
     int levels = 0;
 };
 
 GradLayout grad_layout(int64_t num_rows, int32_t dim, int64_t count, bool sparse) {
     GradLayout l;
-    const int bits = bits_below(num_rows);
-    l.passes = bits == 0 ? 1 : (bits + kDigitBits - 1) / kDigitBits;
-    l.tiles = static_cast<uint32_t>(count > 0 ? (count + kTile - 1) / kTile : 1);
     size_t at = round256(MLXC_WORK_WORDS * sizeof(int64_t));
     auto take = [&at](size_t bytes) {
         const size_t a = at;
         at += round256(bytes);
         return a;
     };
-    for (int b = 0; b < 2; ++b) {
-        l.keys[b] = take(static_cast<size_t>(count) * 4);
-        l.places[b] = take(static_cast<size_t>(count) * 4);
-    }
-    l.counts = take(static_cast<size_t>(l.tiles) * kDigits * 4);
-    l.totals = take(kDigits * 4);
-    l.valid = take(8);
+    l.sort = take(place_sort_bytes(num_rows, count, sparse));
     const int64_t num_out = sparse && count < num_rows ? count : num_rows;
     const int64_t spans = (count + kSpan - 1) / kSpan;
     l.runs = take(static_cast<size_t>(num_out) * sizeof(uint2));
-    l.heads = take(static_cast<size_t>(sparse ? l.tiles : 0) * 4);
-    l.ranks = take(static_cast<size_t>(sparse ? spans : 0) * 4);
     l.first = take(static_cast<size_t>(spans) * dim * 4);
     l.last = take(static_cast<size_t>(spans) * dim * 4);
-    for (int64_t span = kSpan * kFan; l.levels < kMaxLevels && span <= count; span *= kFan)
+    for (int64_t span = kSpan * kFan; l.levels < kMaxLevels && count / span >= kLevelTiles;
+         span *= kFan)
         l.sums[l.levels++] = take(static_cast<size_t>(count / span) * dim * 4);
     l.bytes = at;
     return l;
@@ -630,10 +375,10 @@ int embedding_typed(const Table& table, const Nodes& nodes, int64_t count, float
 
 // The sums' buffers, shared by the kernels that fill and read them.
 struct SumCall {
-    const uint32_t *keys, *places, *valid;
+    SortedPlaces sorted;
     const void* rows;
     int32_t dim;
-    int64_t count, num_out;
+    int64_t count;
     float scale;
     const GradLayout& l;
     void* ws;
@@ -643,38 +388,30 @@ struct SumCall {
 template <typename E, typename O, int N>
 int sums_typed(const SumCall& c, hipStream_t stream) {
     const RowShape shape = row_shape(c.dim, N);
+    const SortedPlaces& p = c.sorted;
     const Parts parts{at<float>(c.ws, c.l.first), at<float>(c.ws, c.l.last)};
     uint2* runs = at<uint2>(c.ws, c.l.runs);
-    const uint32_t* ranks = c.out.ids ? at<const uint32_t>(c.ws, c.l.ranks) : nullptr;
     typename O::S* out = static_cast<typename O::S*>(c.out.p);
-    if (c.count > 0) {
-        hipLaunchKernelGGL((span_sum_kernel<E, O, N>),
-                           row_grid((c.count + kSpan - 1) / kSpan, shape, N), dim3(kBlock), 0,
-                           stream, static_cast<const typename E::S*>(c.rows), c.keys, c.places,
-                           c.valid, ranks, shape, c.scale, parts, runs, out);
-        MLXC_HIP_TRY(hipGetLastError());
-    }
+    hipLaunchKernelGGL((span_sum_kernel<E, O, N>),
+                       row_grid((c.count + kSpan - 1) / kSpan, shape, N), dim3(kBlock), 0, stream,
+                       static_cast<const typename E::S*>(c.rows), p.keys, p.places, p.valid, p.ranks,
+                       shape, c.scale, parts, runs, out);
+    MLXC_HIP_TRY(hipGetLastError());
+    if (c.count <= kSpan) return MLXC_OK;  // one tile
     TileSums tiles{};
     int64_t span = kSpan;
     for (int k = 0; k < c.l.levels; ++k) {
         span *= kFan;
         float* sums = at<float>(c.ws, c.l.sums[k]);
         hipLaunchKernelGGL((tile_sum_kernel<N>), row_grid(c.count / span, shape, N), dim3(kBlock), 0,
-                           stream, c.keys, c.valid, span, k == 0 ? parts.first : tiles.p[k - 1],
+                           stream, p.keys, p.valid, span, k == 0 ? parts.first : tiles.p[k - 1],
                            shape, sums);
         MLXC_HIP_TRY(hipGetLastError());
         tiles.p[k] = sums;
         tiles.levels = k + 1;
     }
-    DeviceInfo info;
-    if (int rc = device_info(info)) return rc;
-    const dim3 finish = row_grid(c.count / kSpan, shape, N);
-    dim3 grid = row_grid(c.num_out, shape, N);
-    const unsigned most = info.cus * kZeroBlocks;
-    grid.x = finish.x + (grid.x < most ? grid.x : most);
-    hipLaunchKernelGGL((row_sum_kernel<O, N>), grid, dim3(kBlock), 0, stream, c.keys, c.valid,
-                       ranks, runs, parts, tiles, shape, finish.x, c.num_out, c.scale, c.out.ids,
-                       out);
+    hipLaunchKernelGGL((run_sum_kernel<O, N>), row_grid(c.count / kSpan, shape, N), dim3(kBlock), 0,
+                       stream, p.keys, p.valid, p.ranks, runs, parts, tiles, shape, c.scale, out);
     MLXC_HIP_TRY(hipGetLastError());
     return MLXC_OK;
 }
@@ -739,56 +476,18 @@ int launch_embedding_grad(const void* rows, int32_t dtype, int32_t dim, const No
                           hipStream_t stream) {
     const bool sparse = out.ids != nullptr;
     const GradLayout l = grad_layout(nodes.num_rows, dim, count, sparse);
-    int64_t* work = static_cast<int64_t*>(workspace);
-    uint32_t* valid = at<uint32_t>(workspace, l.valid);
-    hipLaunchKernelGGL(clear_words_kernel, dim3(1), dim3(kWave), 0, stream, work, MLXC_WORK_WORDS);
-    hipLaunchKernelGGL(clear_words_kernel, dim3(1), dim3(kWave), 0, stream,
-                       at<int64_t>(workspace, l.valid), 1);
-    MLXC_HIP_TRY(hipGetLastError());
     const int64_t num_out =
         sparse ? (count < nodes.num_rows ? count : nodes.num_rows) : nodes.num_rows;
-    if (num_out == 0) return MLXC_OK;
-    uint32_t* counts = at<uint32_t>(workspace, l.counts);
-    uint32_t* totals = at<uint32_t>(workspace, l.totals);
-    uint32_t* runs = at<uint32_t>(workspace, l.runs);
-    const unsigned blocks = l.tiles;
-    int cur = 0;
-    for (int pass = 0; pass < l.passes; ++pass) {
-        const int shift = pass * kDigitBits;
-        const SortIn in{nodes, count, at<uint32_t>(workspace, l.keys[cur]),
-                        at<uint32_t>(workspace, l.places[cur]), valid};
-        const int to = pass == 0 ? 0 : cur ^ 1;
-        uint32_t *keys_out = at<uint32_t>(workspace, l.keys[to]),
-                 *places_out = at<uint32_t>(workspace, l.places[to]);
-        if (pass == 0) {
-            hipLaunchKernelGGL(digit_count_kernel<true>, dim3(blocks), dim3(kBlock), 0, stream, in,
-                               shift, l.tiles, counts, runs, 2 * num_out, work);
-        } else {
-            hipLaunchKernelGGL(digit_count_kernel<false>, dim3(blocks), dim3(kBlock), 0, stream, in,
-                               shift, l.tiles, counts, nullptr, 0, work);
-        }
-        MLXC_HIP_TRY(hipGetLastError());
-        hipLaunchKernelGGL(digit_prefix_kernel, dim3(kDigits), dim3(kBlock), 0, stream, counts,
-                           l.tiles, totals);
-        MLXC_HIP_TRY(hipGetLastError());
-        auto* scatter = pass == 0 ? digit_scatter_kernel<true> : digit_scatter_kernel<false>;
-        hipLaunchKernelGGL(scatter, dim3(blocks), dim3(kBlock), 0, stream, in, shift, l.tiles,
-                           counts, totals, keys_out, places_out, valid);
-        MLXC_HIP_TRY(hipGetLastError());
-        cur = to;
-    }
-    const uint32_t* keys = at<uint32_t>(workspace, l.keys[cur]);
-    const uint32_t* places = at<uint32_t>(workspace, l.places[cur]);
-    if (sparse) {
-        uint32_t* heads = at<uint32_t>(workspace, l.heads);
-        hipLaunchKernelGGL(count_heads_kernel, dim3(blocks), dim3(kBlock), 0, stream, keys, valid,
-                           heads);
-        MLXC_HIP_TRY(hipGetLastError());
-        hipLaunchKernelGGL(list_runs_kernel, dim3(blocks), dim3(kBlock), 0, stream, keys, valid,
-                           heads, at<uint32_t>(workspace, l.ranks), out.ids);
-        MLXC_HIP_TRY(hipGetLastError());
-    }
-    const SumCall c{keys, places, valid, rows, dim, count, num_out, scale, l, workspace, out};
+    // zeros everywhere first, beside the sort's first pass: rows that no place
+    // belongs to keep them
+    const ClearOut clear{out.p, static_cast<size_t>(num_out) * dim * elem_bytes(out.dtype), out.ids,
+                         sparse ? num_out : 0};
+    SortedPlaces sorted;
+    if (int rc = launch_place_sort(nodes, count, clear, static_cast<int64_t*>(workspace),
+                                   at<unsigned char>(workspace, l.sort), sorted, stream))
+        return rc;
+    if (count == 0 || num_out == 0) return MLXC_OK;
+    const SumCall c{sorted, rows, dim, count, scale, l, workspace, out};
     if (dtype == MLXC_FLOAT32) return sums_from<F32>(c, stream);
     if (dtype == MLXC_BFLOAT16) return sums_from<BF16>(c, stream);
     return sums_from<F16>(c, stream);

@@ -44,11 +44,35 @@ inline int pack_width(const void* p, int64_t dim, int64_t stride, size_t esz, in
     return n;
 }
 
+// ---- place_sort.hip
+// Places of a call sorted by node, in ascending order where nodes are equal;
+// places without a node are left out.
+struct SortedPlaces {
+    const uint32_t* keys;    // [valid] nodes
+    const uint32_t* places;  // [valid]
+    const uint32_t* valid;   // one word
+    const uint32_t* ranks;   // per kSpan places, the distinct nodes that start before (or null)
+};
+constexpr int kSpan = 32;
+
+// What the first launch of a sort fills beside it: bytes of zeros, and num_ids
+// ids of -1 (the distinct nodes then replace the first of them).
+struct ClearOut {
+    void* p;
+    size_t bytes;
+    int64_t* ids;
+    int64_t num_ids;
+};
+size_t place_sort_bytes(int64_t num_rows, int64_t count, bool sparse);
+// work receives the call's status (MLXC_WORK_WORDS words).  clear.ids not null:
+// the distinct nodes go there, and ranks are made.
+int launch_place_sort(const Nodes& nodes, int64_t count, const ClearOut& clear, int64_t* work,
+                      void* workspace, SortedPlaces& sorted, hipStream_t stream);
+
 // ---- embedding.hip
 int launch_embedding(const Table& table, const Nodes& nodes, int64_t count, float scale, void* out,
                      int64_t* status, hipStream_t stream);
-// The workspace of a gradient over count places (0: out of range); extra bytes
-// the caller puts at its end, from grad_workspace_end on.
+// The workspace of a gradient over count places.
 size_t grad_workspace_bytes(int64_t num_rows, int32_t dim, int64_t count, bool sparse);
 // Gradient rows `rows` ([count, dim] of dtype, by place), added up by node.
 int launch_embedding_grad(const void* rows, int32_t dtype, int32_t dim, const Nodes& nodes,

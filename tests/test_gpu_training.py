@@ -108,6 +108,51 @@ def test_embedding_grad_large(gpu, V, T, D, dtype, hub, missing, sparse):
     assert torch.equal(got, again[1][:got.shape[0]] if sparse else again)
 
 
+@pytest.mark.parametrize("T", [1, 31, 32, 33, 1023, 1025, 4096, 16383, 16384, 16385, 20481,
+                               262144, 262145, 300000])
+@pytest.mark.parametrize("V", [1, 200, 256, 257, 65537, 1 << 20])
+def test_sort_sizes(gpu, T, V):
+    """Lists on both sides of every limit of the sort: exact sums of small whole numbers,
+    nodes missing and bad, both forms, the status each time."""
+    g = cases.gen(T, V)
+    x = ref.make_nodes(g, (T,), V, 0.1, 0.2)
+    gr = torch.randint(-8, 9, (T, 3), generator=g).float()
+    keep = x >= 0
+    want = torch.zeros(V, 3).index_add_(0, x[keep], gr[keep])
+    ids = torch.unique(x[keep])
+    out = mc.embedding_grad(gr.to(gpu.device), x.to(gpu.device), V)
+    assert torch.equal(out.cpu(), want)
+    got_ids, rows = mc.embedding_grad(gr.to(gpu.device), x.to(gpu.device).int(), V, sparse=True)
+    n = ids.numel()
+    assert torch.equal(got_ids[:n].cpu(), ids) and (got_ids[n:] == -1).all()
+    assert torch.equal(rows[:n].cpu(), want[ids]) and not rows[n:].any()
+    bad = x.clone()
+    bad[T // 2] = V
+    for sparse in (False, True):
+        with pytest.raises(ValueError, match="outside"):
+            mc.embedding_grad(gr.to(gpu.device), bad.to(gpu.device), V, sparse=sparse)
+
+
+def test_gradients_written_anywhere(gpu):
+    """Outputs that start off a 16-byte boundary, between values that stay."""
+    lib = _lib.load()
+    g = cases.gen(13)
+    V, D = 37, 5
+    for T in (300, 20000):
+        x = ref.make_nodes(g, (T,), V, 0.2).to(gpu.device)
+        gr = torch.randn(T, D, generator=g).to(torch.bfloat16).to(gpu.device)
+        want = mc.embedding_grad(gr, x, V)
+        need = lib.mlxc_embedding_grad_workspace_bytes(V, D, T, 0)
+        work = torch.empty(need // 8 + 1, dtype=torch.int64, device=gpu.device)
+        for skip in range(9):
+            buf = torch.full((skip + V * D + 9,), 7.0, dtype=torch.bfloat16, device=gpu.device)
+            assert lib.mlxc_embedding_grad(gr.data_ptr(), D, 1, x.data_ptr(), T, 0, V, 1.0, 0, None,
+                                           buf.data_ptr() + 2 * skip, 1, work.data_ptr(), need,
+                                           torch.cuda.current_stream().cuda_stream) == 0
+            assert torch.equal(buf[skip:skip + V * D].reshape(V, D), want)
+            assert (buf[:skip] == 7).all() and (buf[skip + V * D:] == 7).all()
+
+
 @pytest.mark.parametrize("dtype,D", [(torch.float32, 128), (torch.bfloat16, 128),
                                      (torch.float16, 100), (torch.bfloat16, 64)])
 def test_window_scores_large(gpu, dtype, D):
