@@ -14,7 +14,7 @@
 // Bound by the gather of the rows and the table's stores.  2.65 M rows of 128
 // bfloat16 into a table of 2^20: @GWUS@.  One wavefront a node, place after
 // place, took 1,530 us for the sums alone.
-#include "train_host.h"
+#include "place_sort.h"
 
 namespace mlxc {
 
@@ -296,6 +296,136 @@ __global__ __launch_bounds__(kBlock) void run_sum_kernel(
     }
 }
 
+// ------------------------------------------------------------- few places
+
+// The whole gradient of up to kSmallPlaces places in one launch: a block takes
+// the nodes [block * per, ...) of the table.  It writes their zeros, picks their
+// places out of the whole list, in order, sorts them by node in LDS, and its
+// groups of lanes add up equal shares of them; a run that crosses shares is put
+// together from the parts that the groups left in LDS.
+//
+// Bound by latencies: 12,000 rows of 64 float32 into 2,708 take @FEWUS@ us; sorted
+// by one block and summed up by two more launches 38.
+template <typename E, typename O, int N>
+__global__ __launch_bounds__(kSmallThreads) void few_sum_kernel(
+    const typename E::S* __restrict__ rows, Nodes nodes, int32_t count, int64_t per, int bits,
+    int passes, RowShape shape, float scale, typename O::S* __restrict__ out,
+    int64_t* __restrict__ work) {
+    static_assert(N <= 4, "the parts fit LDS");
+    __shared__ SmallSort l;
+    __shared__ __align__(16) float parts[kSmallThreads][N];  // of the run that enters a share
+    const int t = threadIdx.x, w = t / kWave, lane = t & ((1 << shape.lanes_log) - 1);
+    const int group = t >> shape.lanes_log, groups = kSmallThreads >> shape.lanes_log;
+    const int32_t col = ((blockIdx.y << shape.lanes_log) + lane) * N;
+    const bool active = col < shape.dim;
+    const int64_t lo = blockIdx.x * per;
+    const int64_t hi = lo + per < nodes.num_rows ? lo + per : nodes.num_rows;
+    bool bad = false;
+    int items = (count + kSmallThreads - 1) / kSmallThreads;
+    const int32_t base = w * items * kWave + t % kWave;
+    int32_t v[kItems];
+    load_nodes(v, nodes, base, kWave, count, bad);
+    const float zeros[N] = {};
+    if (active)
+        for (int64_t r = lo + group; r < hi; r += groups)
+            store_pack<O, N>(out + r * shape.dim + col, zeros);
+    // the block's places, in order (wavefront, slot, lane)
+    uint64_t own[kItems];
+    uint32_t in_wave = 0;
+#pragma unroll
+    for (int s = 0; s < kItems; ++s) {
+        own[s] = __ballot(s < items && v[s] >= lo && v[s] < hi);
+        in_wave += __popcll(own[s]);
+    }
+    if (t % kWave == 0) l.tot[w] = in_wave;
+    const int any_bad = __syncthreads_or(bad);
+    if (blockIdx.x == 0 && blockIdx.y == 0 && t < MLXC_WORK_WORDS)
+        work[t] = t == 0 && any_bad ? MLXC_STATUS_BAD_NODE : 0;
+    uint32_t at = 0;
+    int32_t n = 0;
+#pragma unroll
+    for (int k = 0; k < kSmallWaves; ++k) {
+        at += k < w ? l.tot[k] : 0;
+        n += l.tot[k];
+    }
+#pragma unroll
+    for (int s = 0; s < kItems; ++s) {
+        if ((own[s] >> (t % kWave)) & 1) {
+            const uint32_t j = at + lane_rank(own[s]);
+            l.keys[j] = static_cast<uint32_t>(v[s] - lo);
+            l.places[j] = static_cast<uint16_t>(base + s * kWave);
+        }
+        at += __popcll(own[s]);
+    }
+    __syncthreads();
+    if (n == 0) return;
+    for (int pass = 0; pass < passes; ++pass) {
+        uint32_t key[kItems], place[kItems];
+        const uint32_t have = small_entries(l, key, place, n, items);
+        small_pass(l, key, place, have, items, pass * bits, bits, n);
+    }
+    // equal shares, whole batches while there are few
+    const int32_t share = (n + groups - 1) / groups > kBatch ? (n + groups - 1) / groups : kBatch;
+    const int32_t begin = group * share < n ? group * share : n;
+    const int32_t end = n - begin < share ? n : begin + share;
+    uint32_t node = begin < n ? l.keys[begin] : 0;
+    const bool enters = begin > 0 && begin < n && l.keys[begin - 1] == node;
+    bool first = true;  // no run has ended in the share yet
+    float acc[N] = {};
+    for (int32_t i = begin; i < end; i += kBatch) {
+        Pack<typename E::S, N> x[kBatch];
+        uint32_t key[kBatch];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            const int32_t q = i + u < end ? i + u : end - 1;
+            key[u] = l.keys[q];
+            x[u] = *reinterpret_cast<const Pack<typename E::S, N>*>(
+                rows + static_cast<int64_t>(l.places[q]) * shape.dim + (active ? col : 0));
+        }
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) pin(x[u]);
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            if (key[u] != node) {
+                if (first && enters) {
+                    store_pack<F32, N>(parts[t], acc);
+                } else if (active) {
+#pragma unroll
+                    for (int k = 0; k < N; ++k) acc[k] *= scale;
+                    store_pack<O, N>(out + (lo + node) * shape.dim + col, acc);
+                }
+                first = false;
+                node = key[u];
+#pragma unroll
+                for (int k = 0; k < N; ++k) acc[k] = 0.f;
+            }
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                const float y = E::load(x[u].v[k]);
+                acc[k] += i + u < end ? y : 0.f;
+            }
+        }
+    }
+    const bool leaves = begin < n && end < n && l.keys[end] == node;
+    if (first && enters) store_pack<F32, N>(parts[t], acc);
+    __syncthreads();
+    if (begin >= n || (first && enters) || !active) return;
+    if (leaves) {  // the shares after this one, until the run ends
+        int32_t g = group + 1;
+        for (bool more = true; more; ++g) {
+            float x[N];
+            load_pack<F32, N>(x, parts[(g << shape.lanes_log) | lane]);
+#pragma unroll
+            for (int k = 0; k < N; ++k) acc[k] += x[k];
+            const int32_t next = (g + 1) * share;
+            more = next < n && l.keys[next] == node;
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k) acc[k] *= scale;
+    store_pack<O, N>(out + (lo + node) * shape.dim + col, acc);
+}
+
 __global__ void clear_words_kernel(int64_t* words, int n) {
     if (static_cast<int>(threadIdx.x) < n) words[threadIdx.x] = 0;
 }
@@ -376,6 +506,7 @@ int embedding_typed(const Table& table, const Nodes& nodes, int64_t count, float
 // The sums' buffers, shared by the kernels that fill and read them.
 struct SumCall {
     SortedPlaces sorted;
+    Nodes nodes;
     const void* rows;
     int32_t dim;
     int64_t count;
@@ -385,9 +516,34 @@ struct SumCall {
     GradOut out;
 };
 
+// Calls that few_sum_kernel takes.
+bool few_places(int64_t count, const GradOut& out) { return !out.ids && count <= kSmallPlaces; }
+
+template <typename E, typename O, int N>
+int few_launch(const SumCall& c, const RowShape& shape, hipStream_t stream) {
+    DeviceInfo info;
+    if (int rc = device_info(info)) return rc;
+    const int64_t per = (c.nodes.num_rows + info.cus - 1) / info.cus;
+    const int all = bits_below(per);
+    const int passes = (all + kDigitBits - 1) / kDigitBits;
+    const int bits = passes > 0 ? (all + passes - 1) / passes : 1;
+    const int32_t cols = N << shape.lanes_log;
+    hipLaunchKernelGGL((few_sum_kernel<E, O, N>),
+                       dim3(static_cast<unsigned>((c.nodes.num_rows + per - 1) / per),
+                            (shape.dim + cols - 1) / cols),
+                       dim3(kSmallThreads), 0, stream, static_cast<const typename E::S*>(c.rows),
+                       c.nodes, static_cast<int32_t>(c.count), per, bits, passes, shape, c.scale,
+                       static_cast<typename O::S*>(c.out.p), static_cast<int64_t*>(c.ws));
+    MLXC_HIP_TRY(hipGetLastError());
+    return MLXC_OK;
+}
+
 template <typename E, typename O, int N>
 int sums_typed(const SumCall& c, hipStream_t stream) {
     const RowShape shape = row_shape(c.dim, N);
+    if (few_places(c.count, c.out)) {
+        if constexpr (N <= 4) return few_launch<E, O, N>(c, shape, stream);
+    }
     const SortedPlaces& p = c.sorted;
     const Parts parts{at<float>(c.ws, c.l.first), at<float>(c.ws, c.l.last)};
     uint2* runs = at<uint2>(c.ws, c.l.runs);
@@ -423,7 +579,7 @@ int sums_packed(const SumCall& c, hipStream_t stream) {
     constexpr int most = 16 / sizeof(typename E::S);
     const int n = pack_width(c.rows, c.dim, c.dim, sizeof(typename E::S), most);
     const int m = pack_width(c.out.p, c.dim, c.dim, sizeof(typename O::S), n);
-    if (m >= 8) return sums_typed<E, O, most>(c, stream);
+    if (m >= 8 && !few_places(c.count, c.out)) return sums_typed<E, O, most>(c, stream);
     if (m >= 4) return sums_typed<E, O, 4>(c, stream);
     if (m >= 2) return sums_typed<E, O, 2>(c, stream);
     return sums_typed<E, O, 1>(c, stream);
@@ -478,16 +634,17 @@ int launch_embedding_grad(const void* rows, int32_t dtype, int32_t dim, const No
     const GradLayout l = grad_layout(nodes.num_rows, dim, count, sparse);
     const int64_t num_out =
         sparse ? (count < nodes.num_rows ? count : nodes.num_rows) : nodes.num_rows;
-    // zeros everywhere first, beside the sort's first pass: rows that no place
-    // belongs to keep them
-    const ClearOut clear{out.p, static_cast<size_t>(num_out) * dim * elem_bytes(out.dtype), out.ids,
-                         sparse ? num_out : 0};
-    SortedPlaces sorted;
-    if (int rc = launch_place_sort(nodes, count, clear, static_cast<int64_t*>(workspace),
-                                   at<unsigned char>(workspace, l.sort), sorted, stream))
-        return rc;
-    if (count == 0 || num_out == 0) return MLXC_OK;
-    const SumCall c{sorted, rows, dim, count, scale, l, workspace, out};
+    SumCall c{SortedPlaces{}, nodes, rows, dim, count, scale, l, workspace, out};
+    if (!few_places(count, out) || count == 0 || num_out == 0) {
+        // zeros everywhere first, beside the sort's first pass: rows that no
+        // place belongs to keep them
+        const ClearOut clear{out.p, static_cast<size_t>(num_out) * dim * elem_bytes(out.dtype),
+                             out.ids, sparse ? num_out : 0};
+        if (int rc = launch_place_sort(nodes, count, clear, static_cast<int64_t*>(workspace),
+                                       at<unsigned char>(workspace, l.sort), c.sorted, stream))
+            return rc;
+        if (count == 0 || num_out == 0) return MLXC_OK;
+    }
     if (dtype == MLXC_FLOAT32) return sums_from<F32>(c, stream);
     if (dtype == MLXC_BFLOAT16) return sums_from<BF16>(c, stream);
     return sums_from<F16>(c, stream);

@@ -10,15 +10,12 @@
 // counted, and its keys moved through LDS to their places.  A block adds the
 // counts of the tiles before it up itself while there are few of them; else a
 // launch in between does.
-#include "train_host.h"
+#include "place_sort.h"
 
 namespace mlxc {
 
 namespace {
 
-constexpr int kDigitBits = 8;
-constexpr int kDigits = 1 << kDigitBits;
-constexpr int kItems = 16;              // keys a thread
 constexpr int kTile = kBlock * kItems;  // keys a block
 constexpr int kWaveTile = kWave * kItems;
 static_assert(kDigits == kBlock, "one digit a thread");
@@ -27,61 +24,6 @@ static_assert(kDigits == kBlock, "one digit a thread");
 // [tile][digit] array (64 reads a thread, under 3 us); with more they are
 // [digit][tile] and digit_prefix_kernel adds them up.
 constexpr uint32_t kFlatTiles = 64;
-
-constexpr int kSmallThreads = 1024;
-constexpr int kSmallPlaces = kSmallThreads * kItems;
-constexpr int kSmallWaves = kSmallThreads / kWave;
-
-// Exclusive prefix of one value a thread over the block; *total the sum.  `tot`
-// is kThreads / 64 words of LDS.  Contains two barriers.
-template <int kThreads>
-__device__ __forceinline__ uint32_t block_prefix(uint32_t v, uint32_t* tot, uint32_t* total) {
-    const int lane = threadIdx.x % kWave, w = threadIdx.x / kWave;
-    uint32_t inc = v;
-#pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) {
-        const uint32_t u = __shfl_up(inc, o, kWave);
-        if (lane >= o) inc += u;
-    }
-    if (lane == kWave - 1) tot[w] = inc;
-    __syncthreads();
-    uint32_t before = 0, all = 0;
-#pragma unroll
-    for (int k = 0; k < kThreads / kWave; ++k) {
-        if (k < w) before += tot[k];
-        all += tot[k];
-    }
-    *total = all;
-    __syncthreads();
-    return before + inc - v;
-}
-
-// Lanes of the wavefront that are active and hold this lane's digit of `bits`
-// bits.
-__device__ __forceinline__ uint64_t same_digit(uint32_t d, int bits, bool active) {
-    uint64_t peers = __ballot(active);
-#pragma unroll
-    for (int b = 0; b < kDigitBits; ++b) {
-        if (b >= bits) break;
-        const bool bit = (d >> b) & 1;
-        const uint64_t set = __ballot(bit);
-        peers &= bit ? set : ~set;
-    }
-    return peers;
-}
-
-// One slot's rank among the keys of its digit before it in the wavefront's
-// stretch, whose counts so far are cnt[digit].
-__device__ __forceinline__ uint32_t take_rank(uint32_t* cnt, uint32_t d, int bits, bool active) {
-    const uint64_t peers = same_digit(d, bits, active);
-    const uint32_t before = cnt[d];
-    const int r = lane_rank(peers);
-    // the first of the peers writes after all of them have read (one
-    // wavefront: in order)
-    if (active && r == 0) cnt[d] = before + __popcll(peers);
-    __builtin_amdgcn_wave_barrier();
-    return before + r;
-}
 
 // Zeros and -1s by thread `t` of `threads`.
 __device__ __forceinline__ void clear_share(const ClearOut& c, size_t t, size_t threads) {
@@ -111,12 +53,8 @@ __global__ __launch_bounds__(kSmallThreads) void sort_small_kernel(
     Nodes nodes, int32_t count, int bits, int passes, ClearOut clear, uint32_t* __restrict__ keys_out,
     uint32_t* __restrict__ places_out, uint32_t* __restrict__ valid_out,
     uint32_t* __restrict__ ranks, int64_t* __restrict__ work) {
-    __shared__ uint32_t keys[kSmallPlaces];
-    __shared__ uint16_t places[kSmallPlaces];
-    __shared__ uint32_t cnt[kSmallWaves][kDigits];
-    __shared__ uint32_t tot[kSmallWaves];
-    static_assert(kSmallPlaces <= 65536, "places in 16 bits");
-    const int t = threadIdx.x, w = t / kWave, lane = t % kWave;
+    __shared__ SmallSort l;
+    const int t = threadIdx.x;
     if (blockIdx.x > 0) {
         clear.num_ids = 0;  // ids are block 0's
         clear_share(clear, (blockIdx.x - 1) * static_cast<size_t>(kSmallThreads) + t,
@@ -125,65 +63,30 @@ __global__ __launch_bounds__(kSmallThreads) void sort_small_kernel(
     }
     bool bad = false;
     int32_t n = count;
-    uint32_t key[kItems], place[kItems], rank[kItems];
+    uint32_t key[kItems], place[kItems];
     for (int pass = 0; pass < passes; ++pass) {
-        const int from = pass * bits;
-        const uint32_t mask = (1u << bits) - 1;
-        const int items = (n + kSmallThreads - 1) / kSmallThreads;
-        const int32_t base = w * items * kWave + lane;
+        int items;
         uint32_t have = 0;
+        if (pass == 0) {
+            items = (n + kSmallThreads - 1) / kSmallThreads;
+            const int32_t base = t / kWave * items * kWave + t % kWave;
+            int32_t v[kItems];
+            load_nodes(v, nodes, base, kWave, n, bad);
 #pragma unroll
-        for (int s = 0; s < kItems; ++s) {
-            const int32_t i = base + s * kWave;
-            bool ok = s < items && i < n;
-            if (ok) {
-                if (pass == 0) {
-                    const int64_t v = node_at(nodes, i, bad);
-                    ok = v >= 0;
-                    key[s] = static_cast<uint32_t>(v);
-                    place[s] = i;
-                } else {
-                    key[s] = keys[i];
-                    place[s] = places[i];
-                }
+            for (int s = 0; s < kItems; ++s) {
+                have |= static_cast<uint32_t>(s < items && v[s] >= 0) << s;
+                key[s] = v[s];
+                place[s] = base + s * kWave;
             }
-            have |= static_cast<uint32_t>(ok) << s;
+        } else {
+            have = small_entries(l, key, place, n, items);
         }
-        for (int k = t; k < kSmallWaves * kDigits; k += kSmallThreads) (&cnt[0][0])[k] = 0;
-        __syncthreads();
-#pragma unroll
-        for (int s = 0; s < kItems; ++s) {
-            if (s >= items) break;
-            const bool ok = (have >> s) & 1;
-            rank[s] = take_rank(cnt[w], ok ? (key[s] >> from) & mask : 0, bits, ok);
-        }
-        __syncthreads();
-        uint32_t sum = 0;
-        if (t < kDigits)
-            for (int k = 0; k < kSmallWaves; ++k) sum += cnt[k][t];
-        uint32_t all;
-        uint32_t to = block_prefix<kSmallThreads>(sum, tot, &all);
-        if (t < kDigits) {
-            for (int k = 0; k < kSmallWaves; ++k) {
-                const uint32_t c = cnt[k][t];
-                cnt[k][t] = to;
-                to += c;
-            }
-        }
-        n = static_cast<int32_t>(all);
-        __syncthreads();
-#pragma unroll
-        for (int s = 0; s < kItems; ++s) {
-            if (!((have >> s) & 1)) continue;
-            const uint32_t j = cnt[w][(key[s] >> from) & mask] + rank[s];
-            keys[j] = key[s];
-            places[j] = static_cast<uint16_t>(place[s]);
-        }
-        __syncthreads();
+        small_pass(l, key, place, have, items, pass * bits, bits, n);
     }
+    const uint32_t* keys = l.keys;
     for (int32_t i = t; i < n; i += kSmallThreads) {
         keys_out[i] = keys[i];
-        places_out[i] = places[i];
+        places_out[i] = l.places[i];
     }
     const int any_bad = __syncthreads_or(bad);
     if (t == 0) {
@@ -196,7 +99,7 @@ __global__ __launch_bounds__(kSmallThreads) void sort_small_kernel(
     const int32_t per = (n + kSmallThreads - 1) / kSmallThreads, first = t * per;
     uint32_t heads = 0, all;
     for (int32_t i = first; i < first + per && i < n; ++i) heads += i == 0 || keys[i - 1] != keys[i];
-    uint32_t u = block_prefix<kSmallThreads>(heads, tot, &all);
+    uint32_t u = block_prefix<kSmallThreads>(heads, l.tot, &all);
     for (int32_t i = first; i < first + per && i < n; ++i) {
         if (i % kSpan == 0) ranks[i / kSpan] = u;
         if (i == 0 || keys[i - 1] != keys[i]) clear.ids[u++] = keys[i];
@@ -246,13 +149,19 @@ __global__ __launch_bounds__(kBlock) void digit_count_kernel(SortIn in, uint32_t
     const int64_t n = kFirst ? in.count : static_cast<int64_t>(*in.valid);
     const int64_t base = static_cast<int64_t>(blockIdx.x) * kTile;
     bool bad = false;
+    int32_t v[kItems];
+    if (kFirst) {
+        load_nodes(v, in.nodes, base + t, kBlock, n, bad);
+    } else {
 #pragma unroll
-    for (int s = 0; s < kItems; ++s) {
-        const int64_t i = base + s * kBlock + t;
-        if (i >= n) break;
-        const int64_t key = kFirst ? node_at(in.nodes, i, bad) : static_cast<int64_t>(in.keys[i]);
-        if (key >= 0) atomicAdd(&cnt[digit_of(in, static_cast<uint32_t>(key))], 1u);
+        for (int s = 0; s < kItems; ++s) {
+            const int64_t i = base + s * kBlock + t;
+            v[s] = static_cast<int32_t>(n > 0 ? in.keys[i < n ? i : n - 1] : 0);
+        }
     }
+#pragma unroll
+    for (int s = 0; s < kItems; ++s)
+        if (base + s * kBlock + t < n && v[s] >= 0) atomicAdd(&cnt[digit_of(in, v[s])], 1u);
     const int any_bad = __syncthreads_or(bad);
     counts[count_at(t, blockIdx.x, tiles)] = cnt[t];
     if (kFirst && t == 0) bad_tiles[blockIdx.x] = any_bad;
@@ -298,24 +207,25 @@ __global__ __launch_bounds__(kBlock) void digit_scatter_kernel(
     const int64_t base = static_cast<int64_t>(blockIdx.x) * kTile + w * kWaveTile + lane;
     uint32_t key[kItems], place[kItems], rank[kItems];
     uint32_t have = 0;
+    if (kFirst) {
+        bool bad = false;  // (the count has noted it)
+        int32_t v[kItems];
+        load_nodes(v, in.nodes, base, kWave, n, bad);
 #pragma unroll
-    for (int s = 0; s < kItems; ++s) {
-        const int64_t i = base + s * kWave;
-        bool ok = i < n;
-        key[s] = place[s] = 0;
-        if (ok) {
-            if (kFirst) {
-                bool bad = false;
-                const int64_t v = node_at(in.nodes, i, bad);
-                ok = v >= 0;
-                key[s] = static_cast<uint32_t>(v);
-                place[s] = static_cast<uint32_t>(i);
-            } else {
-                key[s] = in.keys[i];
-                place[s] = in.places[i];
-            }
+        for (int s = 0; s < kItems; ++s) {
+            have |= static_cast<uint32_t>(v[s] >= 0) << s;
+            key[s] = v[s];
+            place[s] = static_cast<uint32_t>(base + s * kWave);
         }
-        have |= static_cast<uint32_t>(ok) << s;
+    } else {
+#pragma unroll
+        for (int s = 0; s < kItems; ++s) {
+            const int64_t i = base + s * kWave;
+            const int64_t at = i < n ? i : n - 1;
+            have |= static_cast<uint32_t>(i < n) << s;
+            key[s] = n > 0 ? in.keys[at] : 0;
+            place[s] = n > 0 ? in.places[at] : 0;
+        }
     }
     // digit t's keys in all tiles, and in the tiles before this one
     uint32_t total = 0, before = 0;
@@ -425,12 +335,6 @@ __global__ __launch_bounds__(kBlock) void list_runs_kernel(const uint32_t* __res
 // ------------------------------------------------------------- host side
 
 size_t round256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
-
-int bits_below(int64_t n) {  // bits of n - 1
-    int b = 0;
-    for (uint64_t x = n > 1 ? static_cast<uint64_t>(n - 1) : 0; x; x >>= 1) ++b;
-    return b;
-}
 
 struct SortLayout {
     int passes, bits;  // of a pass's digit
