@@ -70,30 +70,31 @@ __device__ __forceinline__ uint32_t take_rank(uint32_t* cnt, uint32_t d, int bit
     return before + r;
 }
 
-// Nodes base + s * stride (s < kItems) of a list of n, -1 past its end and where
+// Nodes base + s * stride (s < kCount) of a list of n, -1 past its end and where
 // there is none.  Every load is issued before a value is used: past the end the
 // last node again, so that no load sits behind a branch (which the compiler waits
 // at: 12,000 places took 25 us to sort instead of @SMALLUS@).
-__device__ __forceinline__ void load_nodes(int32_t (&v)[kItems], const Nodes& nodes, int64_t base,
+template <int kCount>
+__device__ __forceinline__ void load_nodes(int32_t (&v)[kCount], const Nodes& nodes, int64_t base,
                                            int stride, int64_t n, bool& bad) {
-    int64_t raw[kItems];
+    int64_t raw[kCount];
     if (nodes.wide) {
         const int64_t* p = static_cast<const int64_t*>(nodes.p);
 #pragma unroll
-        for (int s = 0; s < kItems; ++s) {
+        for (int s = 0; s < kCount; ++s) {
             const int64_t i = base + static_cast<int64_t>(s) * stride;
             raw[s] = n > 0 ? p[i < n ? i : n - 1] : -1;
         }
     } else {
         const int32_t* p = static_cast<const int32_t*>(nodes.p);
 #pragma unroll
-        for (int s = 0; s < kItems; ++s) {
+        for (int s = 0; s < kCount; ++s) {
             const int64_t i = base + static_cast<int64_t>(s) * stride;
             raw[s] = n > 0 ? p[i < n ? i : n - 1] : -1;
         }
     }
 #pragma unroll
-    for (int s = 0; s < kItems; ++s) {
+    for (int s = 0; s < kCount; ++s) {
         const bool ok = static_cast<uint64_t>(raw[s]) < static_cast<uint64_t>(nodes.num_rows);
         bad |= !ok && raw[s] != -1;
         v[s] = ok && base + static_cast<int64_t>(s) * stride < n ? static_cast<int32_t>(raw[s]) : -1;

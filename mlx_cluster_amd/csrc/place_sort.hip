@@ -16,9 +16,12 @@ namespace mlxc {
 
 namespace {
 
-constexpr int kTile = kBlock * kItems;  // keys a block
-constexpr int kWaveTile = kWave * kItems;
 static_assert(kDigits == kBlock, "one digit a thread");
+
+// Keys a thread (kPer below), and with them keys a tile: 16, or 4 in lists of so
+// few tiles that a block's own time counts (48,100 places of 2^24 nodes, three
+// passes: @FOURUS@).
+constexpr int kFewItems = 4;
 
 // Tiles up to which a block adds the counts of all tiles itself, from a
 // [tile][digit] array (64 reads a thread, under 3 us); with more they are
@@ -132,7 +135,7 @@ __device__ __forceinline__ size_t count_at(uint32_t digit, uint32_t tile, uint32
 
 // The tiles' digits counted.  The first pass also notes tiles that hold a bad
 // node, and its blocks from `tiles` on clear.
-template <bool kFirst>
+template <bool kFirst, int kPer>
 __global__ __launch_bounds__(kBlock) void digit_count_kernel(SortIn in, uint32_t tiles,
                                                              uint32_t* __restrict__ counts,
                                                              uint32_t* __restrict__ bad_tiles,
@@ -147,20 +150,20 @@ __global__ __launch_bounds__(kBlock) void digit_count_kernel(SortIn in, uint32_t
     cnt[t] = 0;
     __syncthreads();
     const int64_t n = kFirst ? in.count : static_cast<int64_t>(*in.valid);
-    const int64_t base = static_cast<int64_t>(blockIdx.x) * kTile;
+    const int64_t base = static_cast<int64_t>(blockIdx.x) * (kBlock * kPer);
     bool bad = false;
-    int32_t v[kItems];
+    int32_t v[kPer];
     if (kFirst) {
         load_nodes(v, in.nodes, base + t, kBlock, n, bad);
     } else {
 #pragma unroll
-        for (int s = 0; s < kItems; ++s) {
+        for (int s = 0; s < kPer; ++s) {
             const int64_t i = base + s * kBlock + t;
             v[s] = static_cast<int32_t>(n > 0 ? in.keys[i < n ? i : n - 1] : 0);
         }
     }
 #pragma unroll
-    for (int s = 0; s < kItems; ++s)
+    for (int s = 0; s < kPer; ++s)
         if (base + s * kBlock + t < n && v[s] >= 0) atomicAdd(&cnt[digit_of(in, v[s])], 1u);
     const int any_bad = __syncthreads_or(bad);
     counts[count_at(t, blockIdx.x, tiles)] = cnt[t];
@@ -190,36 +193,36 @@ __global__ __launch_bounds__(kBlock) void digit_prefix_kernel(uint32_t* __restri
 // in earlier tiles, and those before it in its tile (wavefront, slot, lane).  A
 // tile's keys are put in order in LDS first, so that a digit's go out together
 // (stored from where they were ranked: 2.65 M places 24 us a pass, so @SCATUS@).
-template <bool kFirst>
+template <bool kFirst, int kPer>
 __global__ __launch_bounds__(kBlock) void digit_scatter_kernel(
     SortIn in, uint32_t tiles, const uint32_t* __restrict__ counts,
     const uint32_t* __restrict__ totals, const uint32_t* __restrict__ bad_tiles,
     uint32_t* __restrict__ keys_out, uint32_t* __restrict__ places_out,
     uint32_t* __restrict__ valid_out, int64_t* __restrict__ work) {
     constexpr int kWaves = kBlock / kWave;
-    __shared__ uint32_t buf_keys[kTile], buf_places[kTile];
+    __shared__ uint32_t buf_keys[(kBlock * kPer)], buf_places[(kBlock * kPer)];
     __shared__ uint32_t cnt[kWaves][kDigits];
     __shared__ uint32_t shift_to[kDigits];  // from a place in the tile to one in the list
     __shared__ uint32_t tot[kWaves];
     const int t = threadIdx.x, w = t / kWave, lane = t % kWave;
     for (int k = 0; k < kWaves; ++k) cnt[k][t] = 0;
     const int64_t n = kFirst ? in.count : static_cast<int64_t>(*in.valid);
-    const int64_t base = static_cast<int64_t>(blockIdx.x) * kTile + w * kWaveTile + lane;
-    uint32_t key[kItems], place[kItems], rank[kItems];
+    const int64_t base = static_cast<int64_t>(blockIdx.x) * (kBlock * kPer) + w * (kWave * kPer) + lane;
+    uint32_t key[kPer], place[kPer], rank[kPer];
     uint32_t have = 0;
     if (kFirst) {
         bool bad = false;  // (the count has noted it)
-        int32_t v[kItems];
+        int32_t v[kPer];
         load_nodes(v, in.nodes, base, kWave, n, bad);
 #pragma unroll
-        for (int s = 0; s < kItems; ++s) {
+        for (int s = 0; s < kPer; ++s) {
             have |= static_cast<uint32_t>(v[s] >= 0) << s;
             key[s] = v[s];
             place[s] = static_cast<uint32_t>(base + s * kWave);
         }
     } else {
 #pragma unroll
-        for (int s = 0; s < kItems; ++s) {
+        for (int s = 0; s < kPer; ++s) {
             const int64_t i = base + s * kWave;
             const int64_t at = i < n ? i : n - 1;
             have |= static_cast<uint32_t>(i < n) << s;
@@ -254,7 +257,7 @@ __global__ __launch_bounds__(kBlock) void digit_scatter_kernel(
         }
     }
 #pragma unroll
-    for (int s = 0; s < kItems; ++s)
+    for (int s = 0; s < kPer; ++s)
         rank[s] = take_rank(cnt[w], digit_of(in, key[s]), in.bits, (have >> s) & 1);
     __syncthreads();
     uint32_t c[kWaves], own = 0;
@@ -273,7 +276,7 @@ __global__ __launch_bounds__(kBlock) void digit_scatter_kernel(
     }
     __syncthreads();
 #pragma unroll
-    for (int s = 0; s < kItems; ++s) {
+    for (int s = 0; s < kPer; ++s) {
         if (!((have >> s) & 1)) continue;
         const uint32_t j = cnt[w][digit_of(in, key[s])] + rank[s];
         buf_keys[j] = key[s];
@@ -291,13 +294,14 @@ __global__ __launch_bounds__(kBlock) void digit_scatter_kernel(
 // ------------------------------------------------------------- distinct nodes
 
 // heads[tile] <- the runs of one node that start in a tile of the sorted places.
+template <int kPer>
 __global__ __launch_bounds__(kBlock) void count_heads_kernel(const uint32_t* __restrict__ keys,
                                                              const uint32_t* __restrict__ valid,
                                                              uint32_t* __restrict__ heads) {
     __shared__ uint32_t tot[kBlock / kWave];
-    const int64_t n = *valid, base = static_cast<int64_t>(blockIdx.x) * kTile;
+    const int64_t n = *valid, base = static_cast<int64_t>(blockIdx.x) * (kBlock * kPer);
     uint32_t c = 0;
-    for (int s = 0; s < kItems; ++s) {
+    for (int s = 0; s < kPer; ++s) {
         const int64_t i = base + s * kBlock + threadIdx.x;
         c += i < n && (i == 0 || keys[i - 1] != keys[i]);
     }
@@ -308,27 +312,28 @@ __global__ __launch_bounds__(kBlock) void count_heads_kernel(const uint32_t* __r
 
 // ... then the runs' nodes, and ranks[p] <- the runs that start before the kSpan
 // places from p * kSpan on.
+template <int kPer>
 __global__ __launch_bounds__(kBlock) void list_runs_kernel(const uint32_t* __restrict__ keys,
                                                            const uint32_t* __restrict__ valid,
                                                            const uint32_t* __restrict__ heads,
                                                            uint32_t* __restrict__ ranks,
                                                            int64_t* __restrict__ ids) {
     __shared__ uint32_t tot[kBlock / kWave];
-    const int64_t n = *valid, base = static_cast<int64_t>(blockIdx.x) * kTile;
+    const int64_t n = *valid, base = static_cast<int64_t>(blockIdx.x) * (kBlock * kPer);
     uint32_t part = 0, before;
     for (uint32_t k = threadIdx.x; k < blockIdx.x; k += kBlock) part += heads[k];
     block_prefix<kBlock>(part, tot, &before);
-    const int64_t first = base + static_cast<int64_t>(threadIdx.x) * kItems;
+    const int64_t first = base + static_cast<int64_t>(threadIdx.x) * kPer;
     uint32_t is_head = 0;
-    for (int s = 0; s < kItems; ++s) {
+    for (int s = 0; s < kPer; ++s) {
         const int64_t i = first + s;
         if (i < n && (i == 0 || keys[i - 1] != keys[i])) is_head |= 1u << s;
     }
     uint32_t all;
     uint32_t u = before + block_prefix<kBlock>(__popc(is_head), tot, &all);
-    static_assert(kSpan % kItems == 0, "a span starts with a thread's places");
+    static_assert(kSpan % kPer == 0, "a span starts with a thread's places");
     if (first % kSpan == 0 && first < n) ranks[first / kSpan] = u;
-    for (int s = 0; s < kItems; ++s)
+    for (int s = 0; s < kPer; ++s)
         if ((is_head >> s) & 1) ids[u++] = keys[first + s];
 }
 
@@ -338,6 +343,7 @@ size_t round256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
 
 struct SortLayout {
     int passes, bits;  // of a pass's digit
+    int items;         // keys a thread
     uint32_t tiles;
     bool small;
     size_t keys[2], places[2], counts, totals, bad, valid, heads, ranks, bytes;
@@ -348,7 +354,9 @@ SortLayout sort_layout(int64_t num_rows, int64_t count, bool sparse) {
     const int all = bits_below(num_rows);
     l.passes = all <= kDigitBits ? 1 : (all + kDigitBits - 1) / kDigitBits;
     l.bits = all == 0 ? 1 : (all + l.passes - 1) / l.passes;
-    l.tiles = static_cast<uint32_t>(count > 0 ? (count + kTile - 1) / kTile : 1);
+    l.items = count <= int64_t{kFlatTiles} * kBlock * kFewItems ? kFewItems : kItems;
+    const int64_t tile = kBlock * l.items;
+    l.tiles = static_cast<uint32_t>(count > 0 ? (count + tile - 1) / tile : 1);
     l.small = count <= kSmallPlaces;
     size_t at = 0;
     auto take = [&at](size_t bytes) {
@@ -382,6 +390,53 @@ unsigned clear_blocks(const ClearOut& c, int threads, int cus) {
     return static_cast<unsigned>(b < 1 ? 1 : b < most ? b : most);
 }
 
+struct Words {  // of the workspace
+    unsigned char* p;
+    uint32_t* operator()(size_t at) const { return reinterpret_cast<uint32_t*>(p + at); }
+};
+
+template <int kPer>
+int launch_passes(const Nodes& nodes, int64_t count, const ClearOut& clear, int64_t* work,
+                  const Words& words, const SortLayout& l, int cus, SortedPlaces& sorted,
+                  hipStream_t stream) {
+    uint32_t* counts = words(l.counts);
+    uint32_t* valid = words(l.valid);
+    int cur = 0;
+    for (int pass = 0; pass < l.passes; ++pass) {
+        const bool first = pass == 0;
+        const SortIn in{nodes, count, words(l.keys[cur]), words(l.places[cur]), valid,
+                        pass * l.bits, l.bits};
+        const int to = first ? 0 : cur ^ 1;
+        const unsigned extra = first ? clear_blocks(clear, kBlock, cus) : 0;
+        auto* count_kernel = first ? digit_count_kernel<true, kPer> : digit_count_kernel<false, kPer>;
+        hipLaunchKernelGGL(count_kernel, dim3(l.tiles + extra), dim3(kBlock), 0, stream, in, l.tiles,
+                           counts, words(l.bad), clear);
+        MLXC_HIP_TRY(hipGetLastError());
+        if (l.tiles > kFlatTiles) {
+            hipLaunchKernelGGL(digit_prefix_kernel, dim3(kDigits), dim3(kBlock), 0, stream, counts,
+                               l.tiles, words(l.totals));
+            MLXC_HIP_TRY(hipGetLastError());
+        }
+        auto* scatter =
+            first ? digit_scatter_kernel<true, kPer> : digit_scatter_kernel<false, kPer>;
+        hipLaunchKernelGGL(scatter, dim3(l.tiles), dim3(kBlock), 0, stream, in, l.tiles, counts,
+                           words(l.totals), words(l.bad), words(l.keys[to]), words(l.places[to]),
+                           valid, work);
+        MLXC_HIP_TRY(hipGetLastError());
+        cur = to;
+    }
+    sorted.keys = words(l.keys[cur]);
+    sorted.places = words(l.places[cur]);
+    if (!sorted.ranks) return MLXC_OK;
+    hipLaunchKernelGGL(count_heads_kernel<kPer>, dim3(l.tiles), dim3(kBlock), 0, stream, sorted.keys,
+                       valid, words(l.heads));
+    MLXC_HIP_TRY(hipGetLastError());
+    hipLaunchKernelGGL(list_runs_kernel<kPer>, dim3(l.tiles), dim3(kBlock), 0, stream, sorted.keys,
+                       valid, words(l.heads), words(l.ranks), clear.ids);
+    MLXC_HIP_TRY(hipGetLastError());
+    return MLXC_OK;
+}
+
 }  // namespace
 
 size_t place_sort_bytes(int64_t num_rows, int64_t count, bool sparse) {
@@ -395,7 +450,7 @@ int launch_place_sort(const Nodes& nodes, int64_t count, const ClearOut& clear, 
     DeviceInfo info;
     if (int rc = device_info(info)) return rc;
     unsigned char* ws = static_cast<unsigned char*>(workspace);
-    auto words = [ws](size_t at) { return reinterpret_cast<uint32_t*>(ws + at); };
+    const Words words{ws};
     uint32_t* valid = words(l.valid);
     uint32_t* ranks = sparse ? words(l.ranks) : nullptr;
     if (l.small) {
@@ -406,40 +461,11 @@ int launch_place_sort(const Nodes& nodes, int64_t count, const ClearOut& clear, 
         sorted = SortedPlaces{words(l.keys[0]), words(l.places[0]), valid, ranks};
         return MLXC_OK;
     }
-    uint32_t* counts = words(l.counts);
-    int cur = 0;
-    for (int pass = 0; pass < l.passes; ++pass) {
-        const bool first = pass == 0;
-        const SortIn in{nodes, count, words(l.keys[cur]), words(l.places[cur]), valid,
-                        pass * l.bits, l.bits};
-        const int to = first ? 0 : cur ^ 1;
-        const unsigned extra = first ? clear_blocks(clear, kBlock, info.cus) : 0;
-        auto* count_kernel = first ? digit_count_kernel<true> : digit_count_kernel<false>;
-        hipLaunchKernelGGL(count_kernel, dim3(l.tiles + extra), dim3(kBlock), 0, stream, in, l.tiles,
-                           counts, words(l.bad), clear);
-        MLXC_HIP_TRY(hipGetLastError());
-        if (l.tiles > kFlatTiles) {
-            hipLaunchKernelGGL(digit_prefix_kernel, dim3(kDigits), dim3(kBlock), 0, stream, counts,
-                               l.tiles, words(l.totals));
-            MLXC_HIP_TRY(hipGetLastError());
-        }
-        auto* scatter = first ? digit_scatter_kernel<true> : digit_scatter_kernel<false>;
-        hipLaunchKernelGGL(scatter, dim3(l.tiles), dim3(kBlock), 0, stream, in, l.tiles, counts,
-                           words(l.totals), words(l.bad), words(l.keys[to]), words(l.places[to]),
-                           valid, work);
-        MLXC_HIP_TRY(hipGetLastError());
-        cur = to;
-    }
-    sorted = SortedPlaces{words(l.keys[cur]), words(l.places[cur]), valid, ranks};
-    if (sparse) {
-        hipLaunchKernelGGL(count_heads_kernel, dim3(l.tiles), dim3(kBlock), 0, stream, sorted.keys,
-                           valid, words(l.heads));
-        MLXC_HIP_TRY(hipGetLastError());
-        hipLaunchKernelGGL(list_runs_kernel, dim3(l.tiles), dim3(kBlock), 0, stream, sorted.keys,
-                           valid, words(l.heads), ranks, clear.ids);
-        MLXC_HIP_TRY(hipGetLastError());
-    }
-    return MLXC_OK;
+    sorted = SortedPlaces{nullptr, nullptr, valid, ranks};
+    return l.items == kItems
+               ? launch_passes<kItems>(nodes, count, clear, work, words, l, info.cus, sorted, stream)
+               : launch_passes<kFewItems>(nodes, count, clear, work, words, l, info.cus, sorted,
+                                          stream);
 }
 
 }  // namespace mlxc

@@ -108,7 +108,7 @@ def test_embedding_grad_large(gpu, V, T, D, dtype, hub, missing, sparse):
     assert torch.equal(got, again[1][:got.shape[0]] if sparse else again)
 
 
-@pytest.mark.parametrize("T", [1, 31, 32, 33, 1023, 1025, 4096, 16383, 16384, 16385, 20481,
+@pytest.mark.parametrize("T", [1, 31, 32, 33, 1023, 1025, 4096, 16383, 16384, 16385, 20481, 65536, 65537,
                                262144, 262145, 300000])
 @pytest.mark.parametrize("V", [1, 200, 256, 257, 65537, 1 << 20])
 def test_sort_sizes(gpu, T, V):
