@@ -308,3 +308,133 @@ def test_workspace_of_exactly_the_size_asked_for(gpu):
         assert torch.equal(out, want) and (buf[need:] == fill).all()
     assert lib.mlxc_embedding_grad(gr.data_ptr(), D, 0, x.data_ptr(), T, 0, V, 1.0, 0, None,
                                    out.data_ptr(), 0, buf.data_ptr(), need - 1, None) == -1
+
+
+def test_example_and_the_host_twins_agree(gpu):
+    """examples/train_embeddings.py on the GPU: the first losses are the host
+    twins' to what float32 adds in a step, and it learns."""
+    import importlib.util
+    import os
+
+    from conftest import REPO
+    spec = importlib.util.spec_from_file_location(
+        "train_embeddings", os.path.join(REPO, "examples", "train_embeddings.py"))
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    kw = dict(nodes=1000, steps=40, batch=500, labelled=0.05, log=lambda *a: None)
+    first, last, right = example.train(device="cuda", **kw)
+    host, _, _ = example.train(device="cpu", **{**kw, "steps": 3})
+    assert all(abs(a - b) < 1e-5 for a, b in zip(first, host))
+    assert max(last) < 0.6 and right > 0.6
+
+
+# ---- the compiled path and the Python layer
+
+
+def test_compiled_path_and_python_layer_agree(gpu, monkeypatch):
+    from mlx_cluster_amd import training
+    if training._fast is None:
+        pytest.skip("the compiled binding is not built")
+    g = cases.gen(14)
+    w = torch.randn(900, 48, generator=g).to(torch.bfloat16).to(gpu.device)
+    x = ref.make_nodes(g, (60, 9), 900, 0.1).to(gpu.device)
+    bad = x.clone()
+    bad[5, 5] = 900
+    sc = mc.window_scores(w, x, 4)
+    m = torch.rand(sc.shape, generator=g).to(gpu.device) < 0.7
+    calls = [
+        lambda: mc.embedding(w, x, scale=2.0), lambda: mc.embedding(w, x.int(), check=False),
+        lambda: mc.embedding_grad(mc.embedding(w, x), x, 900),
+        lambda: mc.embedding_grad(mc.embedding(w, x), x, 900, sparse=True, check=False),
+        lambda: mc.window_scores(w, x, 4), lambda: mc.window_scores(w, x),
+        lambda: mc.window_scores_grad(sc, w, x, 4), lambda: mc.window_scores_grad(sc, w, x, 4, sparse=True),
+        lambda: mc.preference_loss_grad(sc, sc.flip(0), beta=0.3),
+        lambda: mc.preference_loss_grad(sc, sc.flip(0), sc * 0.5, None, chosen_mask=m, normalize=True,
+                                        reduction="sum", label_smoothing=0.1),
+    ]
+    refusals = [
+        lambda: mc.embedding(w, bad), lambda: mc.embedding_grad(mc.embedding(w, x), bad, 900),
+        lambda: mc.window_scores(w, bad, 4), lambda: mc.window_scores_grad(sc, w, bad, 4),
+        lambda: mc.window_scores(w, x, 10), lambda: mc.embedding(w.t(), x.float()),
+        lambda: mc.embedding_grad(mc.embedding(w, x), x[:5], 900),
+        lambda: mc.preference_loss_grad(sc, sc[:3]), lambda: mc.preference_loss_grad(sc, sc, sc[:3]),
+    ]
+
+    def outcome(call):
+        try:
+            out = call()
+            return out if isinstance(out, tuple) else (out,)
+        except (TypeError, ValueError) as e:
+            return type(e), str(e)
+
+    fast = [outcome(c) for c in calls + refusals]
+    monkeypatch.setattr(training, "_fast", None)
+    slow = [outcome(c) for c in calls + refusals]
+    for a, b in zip(fast, slow):
+        assert len(a) == len(b)
+        for p, q in zip(a, b):
+            assert torch.equal(p, q) if isinstance(p, torch.Tensor) else p == q
+    assert all(isinstance(a[0], type) for a in fast[len(calls):])
+
+
+def test_non_finite_rows_stay_where_they_are(gpu):
+    """A row of infinities or NaN reaches the pairs it is in and no others."""
+    g = cases.gen(15)
+    for dtype in cases.FLOATS:
+        for value in (float("nan"), float("inf")):
+            for C in (3, 20):
+                w = torch.randn(200, 64, generator=g)
+                w[7] = value
+                x = torch.randperm(199, generator=g)[:120].reshape(2, 60)
+                x[x == 7] = 199
+                x[0, 30] = 7
+                w = w.to(dtype)
+                s = mc.window_scores(w.to(gpu.device), x.to(gpu.device), C).cpu()
+                hit = torch.zeros(s.shape, dtype=torch.bool)
+                for j in range(60 - C + 1):
+                    for k in range(1, C):
+                        hit[0, j, k - 1] = j == 30 or j + k == 30
+                assert not torch.isfinite(s[hit]).any() and torch.isfinite(s[~hit]).all()
+                gr = torch.randn(s.shape, generator=g)
+                d = mc.window_scores_grad(gr.to(gpu.device), w.to(gpu.device), x.to(gpu.device),
+                                          C).cpu()
+                near = set(x[0, max(0, 30 - C + 1):30 + C].tolist()) - {7}
+                odd = {v for v in range(200) if not torch.isfinite(d[v].float()).all()}
+                assert odd <= near and (odd == near or C > 3)
+                clean = w.clone()
+                clean[7] = 0
+                e = mc.window_scores_grad(gr.to(gpu.device), clean.to(gpu.device),
+                                          x.to(gpu.device), C).cpu()
+                ok = torch.tensor([v not in near for v in range(200)])
+                u = ref.ROUND[dtype][0] * 4
+                assert ((d[ok].float() - e[ok].float()).abs() <= u * (1 + e[ok].float().abs()) * 10).all()
+
+
+def test_largest_width_and_misaligned_arrays(gpu):
+    """Rows that start at any element, wide rows, short and long preference rows off
+    their alignment."""
+    g = cases.gen(16)
+    for dtype in cases.FLOATS:
+        for skip in (1, 2, 3):
+            flat = torch.randn(skip + 50 * 40, generator=g).to(dtype).to(gpu.device)
+            w = flat[skip:].reshape(50, 40)
+            x = ref.make_nodes(g, (6, 11), 50, 0.1).to(gpu.device)
+            same = w.clone()
+            assert torch.equal(mc.embedding(w, x), mc.embedding(same, x))
+            a, b = mc.window_scores(w, x, 5), mc.window_scores(same, x, 5)
+            assert torch.equal(a, b)
+            assert torch.equal(mc.window_scores_grad(a, w, x, 5), mc.window_scores_grad(a, same, x, 5))
+            rows = torch.randn(skip + 66 * 40, generator=g).to(dtype).to(gpu.device)[skip:].reshape(6, 11, 40)
+            assert torch.equal(mc.embedding_grad(rows, x, 50), mc.embedding_grad(rows.clone(), x, 50))
+            for T in (9, 100, 1500):
+                v = torch.randn(skip + 12 * T, generator=g).to(dtype).to(gpu.device)[skip:].reshape(12, T)
+                got = mc.preference_loss_grad(v, v.flip(0), beta=0.01, reduction="sum")
+                want = mc.preference_loss_grad(v.clone(), v.flip(0), beta=0.01, reduction="sum")
+                for p, q in zip(got, want):
+                    assert torch.allclose(p.float(), q.float(), rtol=1e-5 + 4 * ref.ROUND[p.dtype][0],
+                                          atol=1e-6)
+    w = torch.randn(20, 5000, generator=g)
+    x = ref.make_nodes(g, (3, 20), 20, 0.1)
+    for C in (4, 20):
+        want, bound = ref.window_scores(w, x, C, 1.0)
+        ref.close(mc.window_scores(w.to(gpu.device), x.to(gpu.device), C), want, bound)

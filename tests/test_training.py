@@ -270,3 +270,17 @@ def test_half_conversions_of_the_host_twins():
         f = torch.randn(4000, 1, generator=cases.gen(5)) * 10.0**torch.linspace(-42, 39, 4000)[:, None]
         got = mc.embedding_grad(f, torch.arange(4000), 4000, out_dtype=dtype, stream="cpu")
         assert torch.equal(got, f.to(dtype))
+
+
+def test_example_trains_on_the_cpu():
+    """examples/train_embeddings.py: the operators together, on their host twins."""
+    from conftest import REPO
+    import importlib.util
+    spec = importlib.util.spec_from_file_location(
+        "train_embeddings", os.path.join(REPO, "examples", "train_embeddings.py"))
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    first, last, right = example.train(nodes=1000, steps=40, batch=500, labelled=0.05, device="cpu",
+                                       log=lambda *a: None)
+    # losses start at log 2 (no preference); classes by chance are right in one of five
+    assert abs(first[0] - 0.6931) < 0.02 and max(last) < 0.6 and right > 0.6
