@@ -489,13 +489,11 @@ int embedding_typed(const Table& table, const Nodes& nodes, int64_t count, float
                     int64_t* status, hipStream_t stream) {
     const uint32_t packs = table.dim / N;
     const uint32_t inverse = packs > 1 ? 0xffffffffu / packs + 1 : 0;
-    DeviceInfo info;
-    if (int rc = device_info(info)) return rc;
     const bool streamed = static_cast<size_t>(count) * table.dim * sizeof(typename E::S) >
                           (size_t{128} << 20);
     const int64_t chunk = kBlock * (streamed ? 4 : 1);
     int64_t blocks = (count * packs + chunk - 1) / chunk;
-    if (blocks > info.cus * 64) blocks = info.cus * 64;
+    if (blocks > (int64_t{1} << 22)) blocks = int64_t{1} << 22;
     auto* kernel = streamed ? embedding_kernel<E, N, 4, true> : embedding_kernel<E, N, 1, false>;
     hipLaunchKernelGGL(kernel, dim3(blocks), dim3(kBlock), 0, stream,
                        static_cast<const typename E::S*>(table.p), table.row_stride, packs,

@@ -483,6 +483,9 @@ Side side(const mlxc_preference_side& s) {
 }
 
 constexpr int kMaxBlocks = 4096;
+// Short rows: the blocks that are resident together, so that their stretches
+// stay near each other (4.7 M pairs of 9: 204 us, 208 with 4,096).
+constexpr int kShortBlocks = 1536;
 
 enum class Rows { kShort, kGroup, kLong };
 
@@ -522,7 +525,8 @@ Spread spread(const PreferenceCall& c) {
         while ((1 << s.log) < packs) ++s.log;
     }
     const int64_t b = (c.pairs + (kBlock >> s.log) - 1) / (kBlock >> s.log);
-    s.blocks = static_cast<int>(b < 1 ? 1 : b > kMaxBlocks ? kMaxBlocks : b);
+    const int most = s.rows == Rows::kShort ? kShortBlocks : kMaxBlocks;
+    s.blocks = static_cast<int>(b < 1 ? 1 : b > most ? most : b);
     return s;
 }
 
