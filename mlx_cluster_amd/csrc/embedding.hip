@@ -12,8 +12,8 @@
 // atomics, and the order of a sum depends on the places alone.
 //
 // Bound by the gather of the rows and the table's stores.  2.65 M rows of 128
-// bfloat16 (680 MB) into a table of 2^20 (268 MB): 353 us, of which the tiles take
-// 180, the runs that cross them 36, the zeros and the sort 137.  One wavefront a
+// bfloat16 (680 MB) into a table of 2^20 (268 MB): 318 us, of which the tiles take
+// 180, the runs that cross them 36, the zeros and the sort 102.  One wavefront a
 // node, place after place, took 1,530 us for the sums alone.
 #include "place_sort.h"
 
@@ -635,10 +635,11 @@ int launch_embedding_grad(const void* rows, int32_t dtype, int32_t dim, const No
         sparse ? (count < nodes.num_rows ? count : nodes.num_rows) : nodes.num_rows;
     SumCall c{SortedPlaces{}, nodes, rows, dim, count, scale, l, workspace, out};
     if (!few_places(count, out) || count == 0 || num_out == 0) {
-        // zeros everywhere first, beside the sort's first pass: rows that no
-        // place belongs to keep them
-        const ClearOut clear{out.p, static_cast<size_t>(num_out) * dim * elem_bytes(out.dtype),
-                             out.ids, sparse ? num_out : 0};
+        // zeros everywhere first, beside the sort: rows that no place belongs to
+        // keep them
+        const size_t bytes = static_cast<size_t>(num_out) * dim * elem_bytes(out.dtype);
+        const ClearOut clear{out.p, bytes, bytes > (size_t{128} << 20), out.ids,
+                             sparse ? num_out : 0};
         if (int rc = launch_place_sort(nodes, count, clear, static_cast<int64_t*>(workspace),
                                        at<unsigned char>(workspace, l.sort), c.sorted, stream))
             return rc;

@@ -55,11 +55,13 @@ struct SortedPlaces {
 };
 constexpr int kSpan = 32;
 
-// What the first launch of a sort fills beside it: bytes of zeros, and num_ids
-// ids of -1 (the distinct nodes then replace the first of them).
+// What the launches of a sort fill beside it: bytes of zeros (past the caches if
+// streamed), and num_ids ids of -1 (the distinct nodes then replace the first of
+// them).
 struct ClearOut {
     void* p;
     size_t bytes;
+    bool streamed;
     int64_t* ids;
     int64_t num_ids;
 };
