@@ -74,6 +74,57 @@ __global__ __launch_bounds__(kBlock) void embedding_kernel(
     report_bad(bad, status);
 }
 
+// Rows whose packs are smaller than 16 bytes (odd sizes): a thread makes kAll =
+// 16 bytes' worth of the output's elements from pieces of N, of one row and, as
+// dim >= kAll, at most the next, and stores them whole.  1 M rows of 33 float32
+// 99 us with a piece a thread, so 62; 2.74 M of 33 bfloat16 144 and 126.  Bound by
+// the pieces' load instructions.
+template <typename E, int N, bool kStreamed>
+__global__ __launch_bounds__(kBlock) void embedding_odd_kernel(
+    const typename E::S* __restrict__ weight, int64_t row_stride, uint32_t dim, uint32_t inverse,
+    Nodes nodes, int64_t count, float scale, typename E::S* __restrict__ out, int64_t* status) {
+    using S = typename E::S;
+    constexpr int kAll = 16 / sizeof(S);
+    const int64_t total = count * dim;
+    bool bad = false;
+    for (int64_t base = blockIdx.x * static_cast<int64_t>(kBlock * kAll); base < total;
+         base += static_cast<int64_t>(gridDim.x) * kBlock * kAll) {
+        const int64_t row0 = base / dim;  // the same in all threads
+        const uint32_t e = static_cast<uint32_t>(base - row0 * dim) + threadIdx.x * kAll;
+        uint32_t q = __umulhi(e, inverse);
+        if (q * dim > e) --q;  // the inverse is rounded up
+        uint32_t d = e - q * dim;
+        const int64_t i = row0 + q, at = base + threadIdx.x * kAll;
+        const int64_t first = i < count ? node_at(nodes, i, bad) : -1;
+        const int64_t second = i + 1 < count ? node_at(nodes, i + 1, bad) : -1;
+        const S* row = weight + (first < 0 ? 0 : first) * row_stride;
+        const S* next = weight + (second < 0 ? 0 : second) * row_stride;
+        Pack<S, N> x[kAll / N];
+        uint32_t have = 0;
+#pragma unroll
+        for (int k = 0; k < kAll / N; ++k) {
+            const uint32_t here = d + k * N;
+            const bool own = here < dim;
+            // (of no node the table's first row, for a load without a branch)
+            x[k] = *reinterpret_cast<const Pack<S, N>*>(own ? row + here : next + (here - dim));
+            have |= static_cast<uint32_t>(own ? first >= 0 : second >= 0) << k;
+        }
+        Pack<S, kAll> y;
+#pragma unroll
+        for (int k = 0; k < kAll; ++k)
+            y.v[k] = (have >> (k / N)) & 1 ? E::store(E::load(x[k / N].v[k % N]) * scale) : S(0);
+        if (at + kAll <= total) {
+            if constexpr (kStreamed) stream_pack(out + at, y);
+            else *reinterpret_cast<Pack<S, kAll>*>(out + at) = y;
+        } else {
+#pragma unroll
+            for (int k = 0; k < kAll; ++k)
+                if (at + k < total) out[at + k] = y.v[k];
+        }
+    }
+    report_bad(bad, status);
+}
+
 // ------------------------------------------------------------- sums
 
 // The sorted places are added up in tiles of kSpan.  Level 1's tiles hold kFan
@@ -491,6 +542,22 @@ int embedding_typed(const Table& table, const Nodes& nodes, int64_t count, float
     const uint32_t inverse = packs > 1 ? 0xffffffffu / packs + 1 : 0;
     const bool streamed = static_cast<size_t>(count) * table.dim * sizeof(typename E::S) >
                           (size_t{128} << 20);
+    // (1 M rows of 100 bfloat16, two pieces of 8 bytes: 80 us by pieces, 85 whole; of
+    // 50 float32 114 and 85)
+    constexpr int all = 16 / sizeof(typename E::S);
+    if constexpr (N < all && (all / N >= 4 || sizeof(typename E::S) == 4)) {
+        if (table.dim >= all && table.num_rows > 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0) {
+            int64_t grid = (count * table.dim + kBlock * all - 1) / (kBlock * all);
+            if (grid > (int64_t{1} << 22)) grid = int64_t{1} << 22;
+            auto* odd = streamed ? embedding_odd_kernel<E, N, true> : embedding_odd_kernel<E, N, false>;
+            hipLaunchKernelGGL(odd, dim3(grid), dim3(kBlock), 0, stream,
+                               static_cast<const typename E::S*>(table.p), table.row_stride,
+                               static_cast<uint32_t>(table.dim), 0xffffffffu / table.dim + 1, nodes,
+                               count, scale, static_cast<typename E::S*>(out), status);
+            MLXC_HIP_TRY(hipGetLastError());
+            return MLXC_OK;
+        }
+    }
     const int64_t chunk = kBlock * (streamed ? 4 : 1);
     int64_t blocks = (count * packs + chunk - 1) / chunk;
     if (blocks > (int64_t{1} << 22)) blocks = int64_t{1} << 22;
