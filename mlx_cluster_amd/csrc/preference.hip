@@ -301,7 +301,7 @@ __global__ __launch_bounds__(kBlock) void preference_long_kernel(
 // up (rows there an odd number of words apart), the slopes back.
 //
 // Bound by the stream of the values, references and gradients: of 9 float32 a
-// side, 4.7 M pairs (1.06 GB) 213 us, as long as a copy of those bytes.  A group of
+// side, 4.7 M pairs (1.06 GB) 207 us, as long as a copy of those bytes.  A group of
 // lanes a pair, over the packs that its rows touch, takes 531 us: the packs' edges
 // and every lane's own exponentials keep the vector units busy.
 constexpr int kShortLength = 64;

@@ -438,3 +438,32 @@ def test_largest_width_and_misaligned_arrays(gpu):
     for C in (4, 20):
         want, bound = ref.window_scores(w, x, C, 1.0)
         ref.close(mc.window_scores(w.to(gpu.device), x.to(gpu.device), C), want, bound)
+
+
+@pytest.mark.parametrize("dtype", cases.FLOATS)
+@pytest.mark.parametrize("D", [33, 64, 260])
+def test_one_window_gradients_by_hand(gpu, dtype, D):
+    """Walks of one window: pairs without a node count nothing, whatever their gradients hold;
+    a row of NaN reaches the rows it is paired with.  Every product is exact."""
+    g = cases.gen(16, D)
+    V, C = 30, 12
+    w = torch.randint(-4, 5, (V, D), generator=g).float()
+    w[29] = float("nan")
+    x = torch.arange(2 * C).reshape(2, C)
+    x[0, 3], x[0, 7], x[0, 9] = -1, V, 29
+    x = torch.cat([x, x[1:2]])
+    x[2, 0] = -1  # no first node: nothing
+    gr = torch.randint(-2, 3, (3, 1, C - 1), generator=g).float()
+    gr[0, 0, 2], gr[0, 0, 6], gr[2] = float("nan"), float("inf"), float("nan")
+    gr[0, 0, 8] = 1
+    want = torch.zeros(V, D)
+    for n in range(2):
+        for k in range(1, C):
+            a, b = int(x[n, 0]), int(x[n, k])
+            if 0 <= b < V:
+                want[a] += gr[n, 0, k - 1] * w[b]
+                want[b] += gr[n, 0, k - 1] * w[a]
+    got = mc.window_scores_grad(gr.to(gpu.device), w.to(dtype).to(gpu.device), x.to(gpu.device), C,
+                                check=False).cpu().float()
+    assert torch.equal(got.isnan(), want.isnan())
+    assert torch.equal(got.nan_to_num(), want.nan_to_num())
