@@ -454,8 +454,9 @@ __global__ __launch_bounds__(kBlock) void window_rows_grad_kernel(
 // sum over the others, each of theirs the first row times a number.  Nothing for
 // the matrix unit to share: a group of 2^log lanes a walk, a pack of N columns
 // each, kBatch rows in flight.  Bound by the rows' stream: 37,700 windows of 10
-// nodes, 100 float32 (151 MB read, 151 written) 61 us, 96 in tiles of 16 places; whole gradients of 8 to 200,000 such
-// walks of 2 to 32 nodes are 1 to 1.95 times as fast.
+// nodes, 100 float32 (151 MB read, 151 written) 61 us, 96 in tiles of 16 places;
+// whole gradients of 8 to 200,000 such walks of 2 to 32 nodes take 1 to 1 / 1.95
+// of the time.
 template <typename E, int N, bool kStreamed>
 __global__ __launch_bounds__(kBlock) void first_rows_grad_kernel(
     const float* __restrict__ grad, const typename E::S* __restrict__ weight, int64_t row_stride,
