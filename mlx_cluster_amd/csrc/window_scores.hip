@@ -115,7 +115,9 @@ struct Fragment {
     Pack<typename E::S, Matrix<E>::kPer> v[kSteps];
 };
 
-// Values [from, from + kSteps * kStep) of this lane's row, zeros from dim on.
+// Values [from, from + kSteps * kStep) of this lane's row, zeros from dim on
+// (which lies inside these steps wherever they are not all full, also between
+// two of them).
 // kAligned: packs of kPer values lie aligned and fill the rows, and the table
 // has a row; without a branch then, and of no node the first row's.  Else
 // zeros of no node.
@@ -132,7 +134,7 @@ __device__ __forceinline__ void load_fragment(Fragment<E, kSteps>& f,
         const int32_t at = from + s * Matrix<E>::kStep + lane / kTileRows * kPer;
         if (kAligned) {
             f.v[s] = *reinterpret_cast<const Pack<typename E::S, kPer>*>(row + (at < dim ? at : 0));
-            if (dim % Matrix<E>::kStep != 0 && at >= dim) {
+            if (from + kSteps * Matrix<E>::kStep > dim && at >= dim) {
 #pragma unroll
                 for (int q = 0; q < kPer; ++q) f.v[s].v[q] = 0;
             }
