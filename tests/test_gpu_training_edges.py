@@ -8,6 +8,7 @@ import torch
 import mlx_cluster_amd as mc
 import train_cases as cases
 import train_reference as ref
+from mlx_cluster_amd import _lib
 
 pytestmark = pytest.mark.gpu
 
@@ -28,3 +29,55 @@ STEPS = [(torch.float32, D) for D in (48, 80, 96, 112, 144, 176, 208, 240, 272)]
 def test_scores_of_rows_of_whole_steps(gpu, dtype, D, walks):
     cases.check_window_scores(gpu, dtype, D, 50, walks, False, 0.1, 0.7, "plain")
     cases.check_window_scores_grad(gpu, dtype, None, D, 50, walks, True, 0.1, 0.7, False, "plain")
+
+
+def written(V, D, T, dtype, sparse, x, g, skip=0):
+    """The gradient's rows through the C ABI, in memory that held sevens."""
+    lib = _lib.load()
+    flags = _lib.MLXC_GRAD_SPARSE if sparse else 0
+    rows = min(V, T) if sparse else V
+    code = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[dtype]
+    buf = torch.full((skip + rows * D + 8,), 7.0, dtype=dtype, device=x.device)
+    ids = torch.full((rows + 1,), 7, dtype=torch.int64, device=x.device)
+    need = lib.mlxc_embedding_grad_workspace_bytes(V, D, T, flags)
+    work = torch.empty(need // 8 + 1, dtype=torch.int64, device=x.device)
+    rc = lib.mlxc_embedding_grad(
+        g.data_ptr(), D, code, x.data_ptr(), T, 0, V, 1.0, flags, ids.data_ptr() if sparse else None,
+        buf.data_ptr() + skip * buf.element_size(), code, work.data_ptr(), need,
+        torch.cuda.current_stream().cuda_stream)
+    assert rc == 0, _lib.last_error()
+    assert (buf[:skip] == 7).all() and (buf[skip + rows * D:] == 7).all() and int(ids[-1]) == 7
+    return buf[skip:skip + rows * D].reshape(rows, D), ids[:-1]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T", [0, 20000, 70000])
+def test_every_byte_of_a_gradient_is_written(gpu, T, dtype):
+    """No node at all: every size of the rows up to two packs, and around whole pages, at every
+    start that the type allows."""
+    x = torch.full((max(T, 1),), -1, device=gpu.device)
+    g = torch.ones(max(T, 1), device=gpu.device).to(dtype)
+    esz = g.element_size()
+    sizes = list(range(1, 25)) + [4096 * k // esz + d for k in range(1, 9) for d in range(-5, 6)]
+    for n in sizes:
+        for skip in (0, n % (16 // esz)):
+            out, _ = written(n, 1, T, dtype, False, x, g, skip)
+            assert not out.any(), (n, skip, out.nonzero().flatten().tolist()[:4])
+        if T:
+            out, ids = written(n, 1, T, dtype, True, x, g)
+            assert not out.any() and (ids == -1).all(), n
+
+
+@pytest.mark.parametrize("sparse", [False, True])
+@pytest.mark.parametrize("V,D,T,dtype", [
+    (1025, 1, 20000, torch.float32), (3, 1, 20000, torch.float32), (683, 3, 20000, torch.float32),
+    (41, 50, 20000, torch.bfloat16), (82, 50, 20000, torch.bfloat16), (41, 100, 70000, torch.bfloat16),
+    (1229, 10, 20000, torch.bfloat16), (41, 50, 20000, torch.float32)])
+def test_rows_that_no_place_visits_are_zeros(gpu, V, D, T, dtype, sparse):
+    x = torch.arange(T, device=gpu.device) % (V - 2)  # the last two rows: none
+    g = torch.ones(T, D, device=gpu.device).to(dtype)
+    out, ids = written(V, D, T, dtype, sparse, x, g)
+    n = torch.bincount(x, minlength=V).to(dtype)
+    assert torch.equal(out, n.unsqueeze(1).expand(V, D))
+    if sparse:
+        assert ids.tolist() == [*range(V - 2), -1, -1]
