@@ -21,7 +21,10 @@ int node_type(at::ScalarType t) {
     return t == at::kLong ? MLXC_OUT_INT64 : t == at::kInt ? MLXC_OUT_INT32 : -1;
 }
 
-bool recorded(const at::Tensor& t) { return t.requires_grad() && at::GradMode::is_enabled(); }
+// Whether autograd has to see a call of t: to record it, or to refuse a dual tensor.
+bool recorded(const at::Tensor& t) {
+    return (t.requires_grad() && at::GradMode::is_enabled()) || t._fw_grad(0).defined();
+}
 
 // A tensor as it is, on the device that calls run on.
 bool here(const at::Tensor& t, const at::Device& device) {

@@ -6,12 +6,13 @@ node (`embedding`), the scores of skip-gram windows (`window_scores`), a loss
 of preferred against other windows or sequences (`preference_loss`), and their
 gradients (`embedding_grad`, `window_scores_grad`, `preference_loss_grad`).
 
-The first three are differentiable by torch's autograd; the `_grad` functions
-are the same kernels for programs that write their own step.  A node of -1 is
-no node: its row reads as zeros and takes no gradient.  Sums are made in 32
-bits or more and rounded once; the same call gives the same bits every time.
-On the GPU the operators run in HIP kernels, with stream='cpu' in host twins
-that follow the same formulas with 64-bit sums.
+The first three are differentiable by torch's autograd (once, backward; dual
+tensors raise NotImplementedError); the `_grad` functions are the same kernels
+for programs that write their own step.  A node of -1 is no node: its row reads
+as zeros and takes no gradient.  Sums are made in 32 bits or more and rounded
+once; the same call gives the same bits every time.  On the GPU the operators
+run in HIP kernels, with stream='cpu' in host twins that follow the same
+formulas with 64-bit sums.
 """
 from __future__ import annotations
 
@@ -209,8 +210,10 @@ def _autograd_grad(grad: Grad, V: int, device) -> torch.Tensor:
 
 
 def _tracked(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(
-        isinstance(t, torch.Tensor) and t.requires_grad for t in tensors)
+    """Whether autograd has to see a call: one to record, or one of dual tensors,
+    which the functions above refuse (they have no forward-mode derivative)."""
+    return any((t.requires_grad and torch.is_grad_enabled()) or
+               torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def embedding(weight, nodes, *, scale: float = 1.0, sparse_grad: bool = False, check: bool = True,

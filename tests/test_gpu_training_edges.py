@@ -7,6 +7,7 @@ import torch
 
 import mlx_cluster_amd as mc
 import train_cases as cases
+import train_edges as edges
 import train_reference as ref
 from mlx_cluster_amd import _lib
 
@@ -81,3 +82,9 @@ def test_rows_that_no_place_visits_are_zeros(gpu, V, D, T, dtype, sparse):
     assert torch.equal(out, n.unsqueeze(1).expand(V, D))
     if sparse:
         assert ids.tolist() == [*range(V - 2), -1, -1]
+
+
+@pytest.mark.parametrize("grad_mode", [True, False])
+@pytest.mark.parametrize("requires_grad", [False, True])
+def test_dual_tensors_are_refused(gpu, grad_mode, requires_grad):
+    edges.check_dual_tensors(gpu, grad_mode, requires_grad)
