@@ -152,6 +152,16 @@ class _Launch:
         return False
 
 
+def _join_side_stream(stream) -> None:
+    """Torch's current stream waits for a backward's kernels on `stream`: autograd
+    adds their results up and hands them on at once, and leaves no place for the
+    caller to wait (as a forward call on another stream does)."""
+    if isinstance(stream, torch.cuda.Stream):
+        side = _side_stream(stream, stream.device)
+        if side is not None:
+            torch.cuda.current_stream(stream.device).wait_stream(side)
+
+
 # ---------------------------------------------------------------- embedding
 
 def _embedding(weight, nodes, scale: float, check: bool, stream) -> torch.Tensor:
@@ -195,6 +205,7 @@ class _EmbeddingFunction(torch.autograd.Function):
         (nodes,) = ctx.saved_tensors
         V, dtype, device, scale, sparse_grad, stream = ctx.args
         g = _embedding_grad(grad, nodes, V, scale, sparse_grad, dtype, False, stream)
+        _join_side_stream(stream)
         return _autograd_grad(g, V, device), None, None, None, None, None
 
 
@@ -404,6 +415,7 @@ class _WindowScoresFunction(torch.autograd.Function):
         C, scale, sparse_grad, stream = ctx.args
         g = _window_scores_grad(grad, weight, walks, C, scale, sparse_grad, weight.dtype, False,
                                 stream)
+        _join_side_stream(stream)
         return (_autograd_grad(g, weight.shape[0], weight.device),) + (None,) * 6
 
 
@@ -577,6 +589,7 @@ class _PreferenceFunction(torch.autograd.Function):
             with run.uses(slopes, up, *masks, *grads):
                 rc = lib.mlxc_preference_grad(*args, run.handle)
             _lib.check(rc, "preference_loss")
+            _join_side_stream(stream)
         return (*(None if g is None else g.to(d) for g, d in zip(grads, ctx.devices)), None, None)
 
 

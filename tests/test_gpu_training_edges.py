@@ -88,3 +88,67 @@ def test_rows_that_no_place_visits_are_zeros(gpu, V, D, T, dtype, sparse):
 @pytest.mark.parametrize("requires_grad", [False, True])
 def test_dual_tensors_are_refused(gpu, grad_mode, requires_grad):
     edges.check_dual_tensors(gpu, grad_mode, requires_grad)
+
+
+def keep_busy(stream, device):
+    """Some milliseconds of work on `stream`."""
+    with torch.cuda.stream(stream):
+        a = torch.ones(4096, 4096, device=device)
+        for _ in range(4):
+            a = a @ a * 1e-4
+    return a
+
+
+@pytest.mark.parametrize("sparse", [False, True])
+def test_backward_on_another_stream(gpu, sparse):
+    """What autograd does with a gradient comes after the kernels that make it, whatever stream
+    the call named and however long that stream is busy."""
+    g = cases.gen(21)
+    table = torch.randn(3000, 48, generator=g)
+    x = ref.make_nodes(g, (900, 14), 3000, 0.05, 0.1).to(gpu.device)
+    other = ref.make_nodes(g, (900, 14), 3000, 0.0).to(gpu.device)
+    side = torch.cuda.Stream()
+
+    def step(stream, device):
+        # dense: one table in three calls, whose gradients autograd adds up; coalesced: one each
+        leaf = lambda: table.clone().to(device).requires_grad_()
+        leaves = [leaf() for _ in range(3)] if sparse else [leaf()] * 3
+        torch.cuda.synchronize()
+        kw = dict(sparse_grad=sparse, stream=stream)
+        pos = mc.window_scores(leaves[0], x, 5, **kw)
+        neg = mc.window_scores(leaves[1], other, 5, **kw)
+        rows = mc.embedding(leaves[2], x, scale=0.5, **kw)
+        torch.cuda.synchronize()
+        loss = mc.preference_loss(pos, neg, beta=0.5, stream=stream)
+        torch.cuda.synchronize()
+        busy = keep_busy(side, gpu.device)
+        (loss * 7.0 + (rows * rows).sum() * 0.01).backward()
+        return [p.grad.to_dense().cpu() if sparse else p.grad.cpu() for p in leaves]
+
+    want = step(None, gpu.device)
+    for device in (gpu.device, gpu.device, "cpu"):  # a table on the CPU gets its gradient there
+        assert all(torch.equal(a, b) for a, b in zip(step(side, device), want))
+
+
+@pytest.mark.parametrize("mask", [False, True])
+def test_preference_backward_on_another_stream(gpu, mask):
+    g = cases.gen(22)
+    values = [torch.randn(500, n, generator=g).to(gpu.device) for n in (70, 9)]
+    masks = [(torch.rand(v.shape, generator=g) < 0.7).to(gpu.device) if mask else None
+             for v in (values[0].cpu(), values[1].cpu())]
+    side = torch.cuda.Stream()
+
+    def step(stream):
+        leaves = [v.clone().requires_grad_() for v in values]
+        torch.cuda.synchronize()
+        loss = mc.preference_loss(leaves[0] * 2.0, leaves[1] * 3.0, chosen_mask=masks[0],
+                                  rejected_mask=masks[1], stream=stream)
+        if stream is not None:
+            stream.synchronize()
+            busy = keep_busy(stream, gpu.device)
+        loss.backward()
+        return [v.grad.cpu() for v in leaves]
+
+    want = step(None)
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(step(side), want))
