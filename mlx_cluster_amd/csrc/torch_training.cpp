@@ -56,9 +56,12 @@ void check_nodes(const at::Tensor& word, hipStream_t stream, const char* what) {
         throw py::value_error(std::string(what) + ": a node is outside [0, num_nodes) and not -1");
 }
 
+// Sizes that the library takes as 32-bit numbers go to training.py past them.
+bool fits(int64_t size) { return size <= INT32_MAX; }
+
 // Whether weight and nodes are a table and its nodes that the library takes.
 bool table_call(const at::Tensor& weight, const at::Tensor& nodes) {
-    return current(weight) && weight.dim() == 2 && weight.size(1) >= 1 &&
+    return current(weight) && weight.dim() == 2 && weight.size(1) >= 1 && fits(weight.size(1)) &&
            float_type(weight.scalar_type()) >= 0 && node_type(nodes.scalar_type()) >= 0 &&
            here(weight, weight.device()) && here(nodes, weight.device());
 }
@@ -110,7 +113,7 @@ py::object embedding_grad(const at::Tensor& grad, const at::Tensor& nodes, int64
         grad.sizes().slice(0, nodes.dim()) != nodes.sizes())
         return py::none();
     const int64_t D = grad.size(-1), count = nodes.numel();
-    if (D > INT32_MAX) return py::none();
+    if (!fits(D)) return py::none();
     const size_t ws = mlxc_embedding_grad_workspace_bytes(num_nodes, static_cast<int32_t>(D), count,
                                                           sparse ? MLXC_GRAD_SPARSE : 0);
     if (ws == 0) return py::none();
@@ -129,7 +132,7 @@ py::object embedding_grad(const at::Tensor& grad, const at::Tensor& nodes, int64
 
 // The context of a window call's walks (0: the whole walk), or -1.
 int32_t context_of(const at::Tensor& walks, int64_t context_size) {
-    if (walks.dim() != 2 || walks.size(1) < 2 || walks.size(1) > INT32_MAX) return -1;
+    if (walks.dim() != 2 || walks.size(1) < 2 || !fits(walks.size(1))) return -1;
     const int64_t c = context_size ? context_size : walks.size(1);
     return c >= 2 && c <= 32 && c <= walks.size(1) ? static_cast<int32_t>(c) : -1;
 }

@@ -32,6 +32,11 @@ _FLOATS = {torch.float32: _lib.MLXC_FLOAT32, torch.bfloat16: _lib.MLXC_BFLOAT16,
            torch.float16: _lib.MLXC_FLOAT16}
 _NODES = {torch.int64: _lib.MLXC_OUT_INT64, torch.int32: _lib.MLXC_OUT_INT32}
 
+# The library's widest row, and the sizes that it takes as 32-bit numbers: refused
+# here, before they are cut to 32 bits on their way there.
+_MAX_DIM = 65536
+_MAX_SIZE = 2**31 - 1
+
 Grad = Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]
 
 
@@ -64,7 +69,13 @@ def _table(weight) -> torch.Tensor:
     weight = _tensor(weight, _FLOATS, "weight")
     if weight.dim() != 2 or weight.shape[1] < 1:
         raise ValueError("weight must be a 2-D [num_nodes, dim >= 1] tensor")
+    _check_dim(weight.shape[1])
     return weight
+
+
+def _check_dim(dim: int) -> None:
+    if dim > _MAX_DIM:
+        raise ValueError(f"dim must lie in [1, {_MAX_DIM}], got {dim}")
 
 
 def _rows_on(weight: torch.Tensor, device: torch.device) -> torch.Tensor:
@@ -87,6 +98,8 @@ def _walks(walks, context_size) -> Tuple[torch.Tensor, int]:
     walks = _tensor(walks, _NODES, "walks")
     if walks.dim() != 2 or walks.shape[1] < 2:
         raise ValueError("walks must be a 2-D [N, nodes >= 2] tensor")
+    if walks.shape[1] > _MAX_SIZE:
+        raise ValueError(f"walks of at most {_MAX_SIZE} nodes, got {walks.shape[1]}")
     C = walks.shape[1] if context_size is None else _int(context_size, "context_size")
     if not 2 <= C <= min(32, walks.shape[1]):
         raise ValueError("context_size must lie in [2, min(32, nodes per walk)]")
@@ -122,7 +135,7 @@ def _plain(stream, number, *tensors) -> bool:
 
 
 def _plain_int(x) -> bool:
-    return x is None or (type(x) is int and x > 0)
+    return x is None or (type(x) is int and 0 < x <= _MAX_SIZE)
 
 
 class _Launch:
@@ -318,7 +331,8 @@ def embedding_grad(grad, nodes, num_nodes: int, *, scale: float = 1.0, sparse: b
             the call stays asynchronous with check=False.
         out_dtype: of the gradient (default: grad's).
     """
-    if out_dtype is None and type(num_nodes) is int and _plain(stream, scale, grad, nodes):
+    if out_dtype is None and type(num_nodes) is int and 0 <= num_nodes <= _MAX_SIZE and \
+            _plain(stream, scale, grad, nodes):
         res = _fast.embedding_grad(grad, nodes, num_nodes, scale, bool(sparse), bool(check))
         if res is not None:
             return res
@@ -327,10 +341,11 @@ def embedding_grad(grad, nodes, num_nodes: int, *, scale: float = 1.0, sparse: b
     nodes = _tensor(nodes, _NODES, "nodes")
     scale = _number(scale, "scale")
     V = _int(num_nodes, "num_nodes")
-    if V < 0:
-        raise ValueError("num_nodes must be >= 0")
+    if not 0 <= V <= _MAX_SIZE:
+        raise ValueError(f"num_nodes must lie in [0, {_MAX_SIZE}]")
     if grad.dim() != nodes.dim() + 1 or grad.shape[:-1] != nodes.shape or grad.shape[-1] < 1:
         raise ValueError("grad must have shape [*nodes.shape, dim >= 1]")
+    _check_dim(grad.shape[-1])
     return _embedding_grad(grad, nodes, V, scale, bool(sparse), _out_dtype(out_dtype, grad.dtype),
                            check, stream)
 

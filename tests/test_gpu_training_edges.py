@@ -152,3 +152,7 @@ def test_preference_backward_on_another_stream(gpu, mask):
     want = step(None)
     for _ in range(3):
         assert all(torch.equal(a, b) for a, b in zip(step(side), want))
+
+
+def test_sizes_past_32_bits(gpu):
+    edges.check_sizes_past_32_bits(gpu)
