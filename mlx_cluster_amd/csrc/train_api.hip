@@ -4,6 +4,7 @@
 #include <climits>
 #include <cmath>
 #include <new>
+#include <stdexcept>
 
 #include "train_host.h"
 
@@ -155,8 +156,9 @@ int no_throw(F&& body) {
         body();
         return MLXC_OK;
     } catch (const std::bad_alloc&) {
-        return fail(MLXC_ERR_HIP, "out of host memory");
+    } catch (const std::length_error&) {  // more than a vector can ever hold
     }
+    return fail(MLXC_ERR_HIP, "out of host memory");
 }
 
 }  // namespace
