@@ -44,14 +44,19 @@ at::Tensor workspace(size_t bytes, const at::Device& device) {
 hipStream_t current_stream() { return at::hip::getCurrentHIPStream().stream(); }
 
 // Waits for a checked call, whose status is in `word`, and raises for its bits.
+// The wait is for all that is queued before the call too: other Python threads (a
+// data loader's) run meanwhile.
 void check_nodes(const at::Tensor& word, hipStream_t stream, const char* what) {
     int64_t bits = 0;
-    int64_t* h = status_words();
-    if (h) {
-        __atomic_store_n(&h[0], int64_t{0}, __ATOMIC_RELAXED);
-        if (mlxc_publish_status(word.data_ptr(), h, stream) != MLXC_OK) h = nullptr;
+    {
+        const py::gil_scoped_release other_threads_run;
+        int64_t* h = status_words();
+        if (h) {
+            __atomic_store_n(&h[0], int64_t{0}, __ATOMIC_RELAXED);
+            if (mlxc_publish_status(word.data_ptr(), h, stream) != MLXC_OK) h = nullptr;
+        }
+        bits = read_word(word, stream, h, 0);
     }
-    bits = read_word(word, stream, h, 0);
     if (bits & MLXC_STATUS_BAD_NODE)
         throw py::value_error(std::string(what) + ": a node is outside [0, num_nodes) and not -1");
 }

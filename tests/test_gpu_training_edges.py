@@ -1,5 +1,7 @@
 """The training operators' kernels at row sizes, table sizes and ways to call
 that lie between those of test_gpu_training.py."""
+import threading
+import time
 from types import SimpleNamespace
 
 import pytest
@@ -156,3 +158,38 @@ def test_preference_backward_on_another_stream(gpu, mask):
 
 def test_sizes_past_32_bits(gpu):
     edges.check_sizes_past_32_bits(gpu)
+
+
+def test_other_threads_run_while_a_checked_call_waits(gpu):
+    """A checked call waits for all that is queued before it; it does not hold the interpreter."""
+    g = cases.gen(23)
+    w = torch.randn(500, 16, generator=g).to(gpu.device)
+    x = ref.make_nodes(g, (40, 8), 500, 0.1).to(gpu.device)
+    grad = mc.embedding(w, x)
+    scores = mc.window_scores(w, x, 3)
+    a = torch.ones(8192, 8192, device=gpu.device)
+    ticks, stop = [], threading.Event()
+
+    def tick():
+        while not stop.is_set():
+            ticks.append(time.perf_counter())
+            time.sleep(0.001)
+
+    thread = threading.Thread(target=tick)
+    thread.start()
+    try:
+        for call in (lambda: mc.embedding(w, x), lambda: mc.embedding_grad(grad, x, 500),
+                     lambda: mc.window_scores(w, x, 3), lambda: mc.window_scores_grad(scores, w, x, 3)):
+            call()
+            torch.cuda.synchronize()
+            for _ in range(10):  # some tens of milliseconds
+                a = a @ a * 1e-4
+            t0 = time.perf_counter()
+            call()
+            t1 = time.perf_counter()
+            assert t1 - t0 > 0.02  # it waited
+            during = [t for t in ticks if t0 < t < t1]
+            assert len(during) >= 5
+    finally:
+        stop.set()
+        thread.join()
