@@ -645,7 +645,8 @@ int sums_packed(const SumCall& c, hipStream_t stream) {
     constexpr int most = 16 / sizeof(typename E::S);
     const int n = pack_width(c.rows, c.dim, c.dim, sizeof(typename E::S), most);
     const int m = pack_width(c.out.p, c.dim, c.dim, sizeof(typename O::S), n);
-    if (m >= 8 && !few_places(c.count, c.out)) return sums_typed<E, O, most>(c, stream);
+    if constexpr (most == 8 && sizeof(typename O::S) == 2)  // (eight float32 are two packs)
+        if (m >= 8 && !few_places(c.count, c.out)) return sums_typed<E, O, most>(c, stream);
     if (m >= 4) return sums_typed<E, O, 4>(c, stream);
     if (m >= 2) return sums_typed<E, O, 2>(c, stream);
     return sums_typed<E, O, 1>(c, stream);

@@ -553,10 +553,14 @@ int scores_launch(const Table& table, const Walks& walks, float scale, float* sc
     if (int rc = wave_grid(walks.num_walks * split.parts, grid)) return rc;
     const int width = table_width<E>(table);
     const bool aligned = width == Matrix<E>::kPer && table.num_rows > 0;
-    auto* kernel = kLong ? aligned ? window_scores_long_kernel<E, kSteps, kAhead, true>
-                                   : window_scores_long_kernel<E, kSteps, kAhead, false>
-                   : aligned ? window_scores_kernel<E, kSteps, kAhead, true>
-                             : window_scores_kernel<E, kSteps, kAhead, false>;
+    const auto kernel = [aligned] {
+        if constexpr (kLong)
+            return aligned ? window_scores_long_kernel<E, kSteps, kAhead, true>
+                           : window_scores_long_kernel<E, kSteps, kAhead, false>;
+        else
+            return aligned ? window_scores_kernel<E, kSteps, kAhead, true>
+                           : window_scores_kernel<E, kSteps, kAhead, false>;
+    }();
     hipLaunchKernelGGL(kernel, dim3(grid), dim3(kBlock), 0, stream,
                        static_cast<const typename E::S*>(table.p), table.row_stride, table.dim,
                        width, walks, split, scale, scores, status);
