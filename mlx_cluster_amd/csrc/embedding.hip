@@ -486,15 +486,26 @@ __global__ void clear_words_kernel(int64_t* words, int n) {
 
 size_t round256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
 
-// The workspace: the header, the sort's part, then the sums'.
+// Calls that few_sum_kernel takes, which works in LDS.
+bool few_places(int64_t num_rows, int64_t count, bool sparse) {
+    return !sparse && num_rows > 0 && count > 0 && count <= kSmallPlaces;
+}
+
+// The workspace: the header, and for more places the sort's part, then the sums'.
 struct GradLayout {
-    size_t sort, runs, first, last, sums[kMaxLevels], bytes;
+    size_t sort = 0, runs = 0, first = 0, last = 0, sums[kMaxLevels] = {}, bytes = 0;
     int levels = 0;
+    bool few = false;
 };
 
 GradLayout grad_layout(int64_t num_rows, int32_t dim, int64_t count, bool sparse) {
     GradLayout l;
     size_t at = round256(MLXC_WORK_WORDS * sizeof(int64_t));
+    l.few = few_places(num_rows, count, sparse);
+    if (l.few) {
+        l.bytes = at;
+        return l;
+    }
     auto take = [&at](size_t bytes) {
         const size_t a = at;
         at += round256(bytes);
@@ -582,9 +593,6 @@ struct SumCall {
     GradOut out;
 };
 
-// Calls that few_sum_kernel takes.
-bool few_places(int64_t count, const GradOut& out) { return !out.ids && count <= kSmallPlaces; }
-
 template <typename E, typename O, int N>
 int few_launch(const SumCall& c, const RowShape& shape, hipStream_t stream) {
     DeviceInfo info;
@@ -607,7 +615,7 @@ int few_launch(const SumCall& c, const RowShape& shape, hipStream_t stream) {
 template <typename E, typename O, int N>
 int sums_typed(const SumCall& c, hipStream_t stream) {
     const RowShape shape = row_shape(c.dim, N);
-    if (few_places(c.count, c.out)) {
+    if (c.l.few) {
         if constexpr (N <= 4) return few_launch<E, O, N>(c, shape, stream);
     }
     const SortedPlaces& p = c.sorted;
@@ -646,7 +654,7 @@ int sums_packed(const SumCall& c, hipStream_t stream) {
     const int n = pack_width(c.rows, c.dim, c.dim, sizeof(typename E::S), most);
     const int m = pack_width(c.out.p, c.dim, c.dim, sizeof(typename O::S), n);
     if constexpr (most == 8 && sizeof(typename O::S) == 2)  // (eight float32 are two packs)
-        if (m >= 8 && !few_places(c.count, c.out)) return sums_typed<E, O, most>(c, stream);
+        if (m >= 8 && !c.l.few) return sums_typed<E, O, most>(c, stream);
     if (m >= 4) return sums_typed<E, O, 4>(c, stream);
     if (m >= 2) return sums_typed<E, O, 2>(c, stream);
     return sums_typed<E, O, 1>(c, stream);
@@ -702,7 +710,7 @@ int launch_embedding_grad(const void* rows, int32_t dtype, int32_t dim, const No
     const int64_t num_out =
         sparse ? (count < nodes.num_rows ? count : nodes.num_rows) : nodes.num_rows;
     SumCall c{SortedPlaces{}, nodes, rows, dim, count, scale, l, workspace, out};
-    if (!few_places(count, out) || count == 0 || num_out == 0) {
+    if (!l.few) {
         // zeros everywhere first, beside the sort: rows that no place belongs to
         // keep them
         const size_t bytes = static_cast<size_t>(num_out) * dim * elem_bytes(out.dtype);
