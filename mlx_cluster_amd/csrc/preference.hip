@@ -483,9 +483,9 @@ Side side(const mlxc_preference_side& s) {
 }
 
 constexpr int kMaxBlocks = 4096;
-// Short rows: the blocks that are resident together, so that their stretches
-// stay near each other (4.7 M pairs of 9: 204 us, 208 with 4,096).
-constexpr int kShortBlocks = 1536;
+// Short rows: the blocks that are resident together (their LDS), so that their
+// stretches stay near each other (4.7 M pairs of 9: 204 us, 208 with 4,096 blocks).
+constexpr int kShortBlocksPerUnit = 6;
 
 enum class Rows { kShort, kGroup, kLong };
 
@@ -500,8 +500,8 @@ struct Spread {
 // The kernel goes by the longer side.  Up to kShortLength values the rows pass
 // through LDS; a row that more than a wavefront's packs reach takes half a
 // block; a group of lanes takes those between.
-Spread spread(const PreferenceCall& c) {
-    Spread s{};
+int spread(const PreferenceCall& c, Spread& s) {
+    s = Spread{};
     const size_t esz = elem_bytes(c.dtype);
     const int64_t per = 16 / esz;
     int64_t longest = 1;
@@ -525,9 +525,14 @@ Spread spread(const PreferenceCall& c) {
         while ((1 << s.log) < packs) ++s.log;
     }
     const int64_t b = (c.pairs + (kBlock >> s.log) - 1) / (kBlock >> s.log);
-    const int most = s.rows == Rows::kShort ? kShortBlocks : kMaxBlocks;
+    int most = kMaxBlocks;
+    if (s.rows == Rows::kShort) {
+        DeviceInfo info;
+        if (int rc = device_info(info)) return rc;
+        if (info.cus * kShortBlocksPerUnit < most) most = info.cus * kShortBlocksPerUnit;
+    }
     s.blocks = static_cast<int>(b < 1 ? 1 : b > most ? most : b);
-    return s;
+    return MLXC_OK;
 }
 
 template <typename E, int kPer>
@@ -552,7 +557,8 @@ template <typename E>
 int loss_typed(const PreferenceCall& c, float* loss, float* rewards, float* slopes, void* workspace,
                hipStream_t stream) {
     constexpr int per = 16 / sizeof(typename E::S);
-    const Spread s = spread(c);
+    Spread s;
+    if (int rc = spread(c, s)) return rc;
     return s.packed ? loss_launch<E, per>(c, s, loss, rewards, slopes, workspace, stream)
                     : loss_launch<E, 1>(c, s, loss, rewards, slopes, workspace, stream);
 }
@@ -561,7 +567,8 @@ template <typename E>
 int grad_typed(const PreferenceCall& c, const float* slopes, const float* upstream,
                hipStream_t stream) {
     constexpr int per = 16 / sizeof(typename E::S);
-    const Spread s = spread(c);
+    Spread s;
+    if (int rc = spread(c, s)) return rc;
     // short rows: their packs a group
     const int log = s.rows == Rows::kShort ? s.log + 2 : s.log;
     const int64_t b = (c.pairs + (kBlock >> log) - 1) / (kBlock >> log);
