@@ -193,3 +193,41 @@ def test_other_threads_run_while_a_checked_call_waits(gpu):
     finally:
         stop.set()
         thread.join()
+
+
+def test_non_finite_rows_reach_every_place_they_are_paired_with(gpu):
+    """The gradient of every place that is in a pair with a row of NaN or infinities is one too,
+    over several tiles of places, and no other is."""
+    g = cases.gen(15)
+    for dtype in cases.FLOATS:
+        for value in (float("nan"), float("inf")):
+            for M, C, at in ((60, 20, 30), (60, 3, 30), (90, 32, 47), (70, 17, 5), (61, 32, 60)):
+                w = torch.randn(200, 64, generator=g)
+                w[7] = value
+                w = w.to(dtype)
+                x = torch.randperm(199, generator=g)[:M].unsqueeze(0)
+                x[x == 7] = 199
+                x[0, at] = 7
+                gr = 1.0 + torch.rand(1, M - C + 1, C - 1, generator=g)
+                pairs = {o for o in range(M)
+                         if 0 < abs(o - at) < C and min(o, at) < M - C + 1}
+                d = mc.window_scores_grad(gr.to(gpu.device), w.to(gpu.device), x.to(gpu.device),
+                                          C).cpu()
+                odd = {v for v in range(200) if not torch.isfinite(d[v].float()).all()}
+                assert odd == {int(x[0, o]) for o in pairs}
+
+
+@pytest.mark.parametrize("D,dtype", [(256, torch.float32), (260, torch.bfloat16), (33, torch.float16)])
+@pytest.mark.parametrize("hub", [0.0, 0.5, 1.0])
+def test_short_lists_of_hubs(gpu, hub, D, dtype):
+    """The largest list that one launch takes, all or half of it one node, with wide rows of
+    values that round."""
+    T, V = 16384, 700
+    g = cases.gen(T, D)
+    x = ref.make_nodes(g, (T,), V, 0.0, hub)
+    gr = torch.randn(T, D, generator=g).to(dtype)
+    got = mc.embedding_grad(gr.to(gpu.device), x.to(gpu.device), V).cpu()
+    total = torch.zeros(V, D, dtype=torch.float64).index_add_(0, x, gr.double())
+    size = torch.zeros(V, D, dtype=torch.float64).index_add_(0, x, gr.double().abs())
+    n = torch.bincount(x, minlength=V).double().unsqueeze(1)
+    ref.close(got, *ref.stored(total, (n + 4) * ref.U32 * size, dtype))
