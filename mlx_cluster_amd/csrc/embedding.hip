@@ -8,8 +8,12 @@
 // of thousands of times, so the sorted places are added up in tiles of 32, each
 // by one group of lanes whatever runs it holds; a run that crosses tiles is put
 // together from its tiles' parts, a hub's from sums of 16 tiles, of 16 of these,
-// and so on.  So no lane adds more than a few dozen rows, nothing is added with
-// atomics, and the order of a sum depends on the places alone.
+// and so on.  A lane's chain of float32 additions is then 32 rows, and for a run
+// that crosses tiles at most 30 parts a level and about 510 of the highest (the
+// next level is built from 32 tiles on).  In lists of up to 16,384 places, which
+// one launch takes, a lane adds up its share of a block's places: 8, or of hubs up to
+// 1,024 (rows of more than 32 packs).  Nothing is added with atomics, and the order
+// of a sum depends on the places alone.
 //
 // Bound by the gather of the rows and the table's stores.  2.65 M rows of 128
 // bfloat16 (680 MB) into a table of 2^20 (268 MB): 318 us, of which the tiles take

@@ -6,10 +6,10 @@
 // needs written everywhere (zeros, ids of -1), by blocks of their own.
 //
 // Up to 16,384 places are sorted by one block in LDS; longer lists in passes of
-// up to 8 bits, two launches each: the digits of every tile of 4,096 are
-// counted, and its keys moved through LDS to their places.  A block adds the
-// counts of the tiles before it up itself while there are few of them; else a
-// launch in between does.
+// up to 8 bits, two launches each: the digits of every tile are counted, 4,096
+// places or (in lists of up to 65,536) 1,024, and its keys moved through LDS to their
+// places.  A block adds the counts of the tiles before it up itself while there are
+// few of them; else a launch in between does.
 #include "place_sort.h"
 
 namespace mlxc {
