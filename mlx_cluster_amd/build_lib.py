@@ -141,6 +141,9 @@ KERNEL_SOURCES = {
     "node2vec_walk": ["walk_device.h", "walk_host.h", "csr_check.h", "prep_kernels.hip", "node2vec_walk.hip"],
     "csr_build": ["walk_device.h", "walk_host.h", "block_sort.h", "csr_build.hip"],
     "context_windows": ["walk_device.h", "walk_host.h", "windows.hip"],
+    "training_operators": ["walk_host.h", "train_host.h", "train_device.h", "place_sort.h",
+                           "place_sort.hip", "embedding.hip", "window_scores.hip",
+                           "preference.hip", "mlxc_train.h"],
     # the probe's kernel uses nothing from the walk headers (its launcher only
     # their host helpers)
     "gather_probe": ["gather_probe.hip"],
